@@ -20,6 +20,7 @@ LIB_DIR = os.path.join(PKG, "lib")
 CORE_LIB = os.path.join(LIB_DIR, "libdataflow.so")
 CONFIG_LIB = os.path.join(LIB_DIR, "libdataflow_hip_config.so")
 KERNELS = os.path.join(LIB_DIR, "dataflow_kernels_gfx950.hsaco")
+SCORE_KERNELS = os.path.join(LIB_DIR, "dataflow_scores_gfx950.hsaco")
 MATMUL_LIB = os.path.join(LIB_DIR, "libdataflow_hipblaslt.so")
 NOALLOC_LIB = os.path.join(LIB_DIR, "libdataflow_noalloc.so")
 # measurement only: streaming copies bench.py times as the memory ceiling
@@ -170,6 +171,13 @@ def _declare(L):
     L.submit_softmax.argtypes = [h, s, i, i, i, i, vp, vp]
     L.submit_cross_entropy_loss.argtypes = [h, s, i, i, i, vp, vp]
     L.submit_softmax_cross_entropy_loss.argtypes = [h, s, i, i, i, vp, vp, vp, vp]
+    L.register_native_score_ops.argtypes = [_H, ctypes.c_char_p, ctypes.c_char_p]
+    for f in (L.dataflow_token_logprobs_workspace, L.dataflow_distillation_loss_workspace):
+        f.restype = u64
+        f.argtypes = [i, i, i, i]
+    L.submit_token_logprobs.argtypes = [h, s, i, i, i, u64, f32, i, i, vp, vp, vp, vp, vp, vp, vp, u64, vp]
+    L.submit_token_logprobs_bwd.argtypes = [h, s, i, i, i, u64, u64, f32, i, vp, vp, vp, vp, vp, vp, vp]
+    L.submit_distillation_loss.argtypes = [h, s, i, i, i, u64, u64, f32, i, vp, vp, vp, vp, vp, vp, vp, u64, vp]
 
 
 _noalloc = None
@@ -218,9 +226,10 @@ def header_bytes(sk):
 
 
 class Handle:
-    """A Dataflow_Handle on one AMD GPU (COMPUTE_HSA) with the native ops registered."""
+    """A Dataflow_Handle on one AMD GPU (COMPUTE_HSA) with the native ops registered,
+    and on request the external matmul and the scoring ops."""
 
-    def __init__(self, device_id=0, num_streams=1, register=True, matmul=False):
+    def __init__(self, device_id=0, num_streams=1, register=True, matmul=False, scores=False):
         self.h = DataflowHandle()
         L = lib()
         if L.init_dataflow_handle(ctypes.byref(self.h), COMPUTE_HSA, device_id, 0, 0, num_streams, None, None) != 0:
@@ -237,6 +246,11 @@ class Handle:
             if L.register_external_matmul(ctypes.byref(self.h), MATMUL_LIB.encode()) != 1:
                 raise RuntimeError("register_external_matmul failed (%s)" % MATMUL_LIB)
             self.num_registered += 1
+        if scores:
+            n = L.register_native_score_ops(ctypes.byref(self.h), SCORE_KERNELS.encode(), CONFIG_LIB.encode())
+            if n <= 0:
+                raise RuntimeError("register_native_score_ops failed (%d)" % n)
+            self.num_registered += n
 
     @property
     def ref(self):
@@ -424,3 +438,37 @@ def submit_cross_entropy_loss(handle, stream_id, bwd_dt, n_rows, n_cols, pred_lo
 def submit_softmax_cross_entropy_loss(handle, stream_id, dt, n_rows, n_cols, logits, labels, loss, mean_loss):
     return lib().submit_softmax_cross_entropy_loss(_h(handle), stream_id, dt, n_rows, n_cols, logits, labels,
                                                    loss, mean_loss)
+
+
+# ---- scoring ops (include/dataflow_score_ops.h; no reference counterpart) ----
+
+def token_logprobs_workspace(dt, n_rows, n_cols, top_k):
+    """Workspace bytes of submit_token_logprobs for these sizes (0: none needed)."""
+    return lib().dataflow_token_logprobs_workspace(dt, n_rows, n_cols, top_k)
+
+
+def distillation_loss_workspace(dt, n_rows, n_cols, top_k):
+    """Workspace bytes of submit_distillation_loss for these sizes (0: none needed)."""
+    return lib().dataflow_distillation_loss_workspace(dt, n_rows, n_cols, top_k)
+
+
+def submit_token_logprobs(handle, stream_id, dt, n_rows, n_cols, row_stride, scale, tokens_per_row, top_k, logits, tokens,
+                          logprobs, entropy, lse, top_ids, top_logprobs, workspaceBytes=0, workspace=None):
+    """Log-probabilities of given tokens, entropy, log-sum-exp and the top_k likeliest columns of each row."""
+    return lib().submit_token_logprobs(_h(handle), stream_id, dt, n_rows, n_cols, row_stride, scale, tokens_per_row, top_k,
+                                       logits, tokens, logprobs, entropy, lse, top_ids, top_logprobs, workspaceBytes, workspace)
+
+
+def submit_token_logprobs_bwd(handle, stream_id, dt, n_rows, n_cols, row_stride, grad_stride, scale, tokens_per_row, logits,
+                              tokens, lse, entropy, d_logprobs, d_entropy, dlogits):
+    """The logits' gradient from those of submit_token_logprobs' log-probabilities and entropy."""
+    return lib().submit_token_logprobs_bwd(_h(handle), stream_id, dt, n_rows, n_cols, row_stride, grad_stride, scale,
+                                           tokens_per_row, logits, tokens, lse, entropy, d_logprobs, d_entropy, dlogits)
+
+
+def submit_distillation_loss(handle, stream_id, dt, n_rows, n_cols, row_stride, grad_stride, scale, top_k, logits, teacher_ids,
+                             teacher_logits, row_weights, loss, mean_loss, dlogits, workspaceBytes=0, workspace=None):
+    """Distillation loss against a teacher's top logits, and (dlogits given) the logits' gradient."""
+    return lib().submit_distillation_loss(_h(handle), stream_id, dt, n_rows, n_cols, row_stride, grad_stride, scale, top_k,
+                                          logits, teacher_ids, teacher_logits, row_weights, loss, mean_loss, dlogits,
+                                          workspaceBytes, workspace)

@@ -5,6 +5,7 @@ Outputs (in-tree, under dataflow_lib_amd/lib/):
                                  submit_* op API and the HIP backend of Dataflow_Handle
   libdataflow_hip_config.so      launch configurations (dlopen'ed by the backend)
   dataflow_kernels_gfx950.hsaco  gfx950 code object (hipModuleLoad'ed by the backend)
+  dataflow_scores_gfx950.hsaco   gfx950 code object of the scoring ops (register_native_score_ops)
   libdataflow_hipblaslt.so       the external matmul op on hipBLASLt (register_external_matmul)
   libdataflow_noalloc.so         the allocation-free entry point (include/dataflow_noalloc.h):
                                  host code and its gfx950 kernels in one HIP fat binary
@@ -28,6 +29,7 @@ CC = os.environ.get("CC", "gcc")
 
 ARCH = "gfx950"
 KERNELS_OUT = os.path.join(LIB, "dataflow_kernels_gfx950.hsaco")
+SCORES_OUT = os.path.join(LIB, "dataflow_scores_gfx950.hsaco")
 CORE_OUT = os.path.join(LIB, "libdataflow.so")
 CONFIG_OUT = os.path.join(LIB, "libdataflow_hip_config.so")
 MATMUL_OUT = os.path.join(LIB, "libdataflow_hipblaslt.so")
@@ -38,7 +40,7 @@ CXX = os.environ.get("CXX", "g++")
 
 C_FLAGS = ["-O2", "-fPIC", "-std=gnu11", "-Wall", "-Wextra", "-Werror=format", "-Wno-unused-parameter", "-Wno-stringop-truncation",
            "-D__HIP_PLATFORM_AMD__", "-I", INCLUDE, "-I", os.path.join(CSRC, "kernels"),
-           "-I", os.path.join(ROCM, "include")]
+           "-I", os.path.join(CSRC, "scores"), "-I", os.path.join(ROCM, "include")]
 HIP_LINK = ["-L", os.path.join(ROCM, "lib"), "-lamdhip64", "-Wl,-rpath," + os.path.join(ROCM, "lib")]
 # packed fp32 VALU forms are kept out of every code object
 HIP_FLAGS = ["--offload-arch=" + ARCH, "-O3", "--genco", "-std=c++17",
@@ -82,6 +84,7 @@ def build(verbose=False):
         raise RuntimeError("hipcc not found at %s" % HIPCC)
     os.makedirs(LIB, exist_ok=True)
     _atomic(KERNELS_OUT, lambda o: _run([HIPCC] + HIP_FLAGS + [os.path.join(CSRC, "kernels", "dataflow_kernels.hip"), "-o", o], verbose))
+    _atomic(SCORES_OUT, lambda o: _run([HIPCC] + HIP_FLAGS + [os.path.join(CSRC, "scores", "score_kernels.hip"), "-o", o], verbose))
     _atomic(CORE_OUT, lambda o: _run([CC, "-shared"] + C_FLAGS + _sources("core", "ops", "backend/hip") +
                                       ["-o", o, "-lcrypto", "-ldl", "-lpthread"] + HIP_LINK, verbose))
     _atomic(CONFIG_OUT, lambda o: _run([CC, "-shared"] + C_FLAGS + _sources("config") +
@@ -98,7 +101,7 @@ def build(verbose=False):
     _atomic(SUBMIT_COST_OUT, lambda o: _run([CC] + C_FLAGS + [os.path.join(CSRC, "bench", "submit_cost.c"), "-o", o,
                                              "-L", LIB, "-ldataflow", "-Wl,-rpath,$ORIGIN"] + HIP_LINK, verbose))
     _atomic(BENCH_COPY_OUT, lambda o: _run([HIPCC] + HIP_FLAGS + [os.path.join(CSRC, "bench", "stream_copy.hip"), "-o", o], verbose))
-    return {"kernels": KERNELS_OUT, "core": CORE_OUT, "config": CONFIG_OUT, "matmul": MATMUL_OUT,
+    return {"kernels": KERNELS_OUT, "scores": SCORES_OUT, "core": CORE_OUT, "config": CONFIG_OUT, "matmul": MATMUL_OUT,
             "noalloc": NOALLOC_OUT, "bench_copy": BENCH_COPY_OUT, "submit_cost": SUBMIT_COST_OUT}
 
 

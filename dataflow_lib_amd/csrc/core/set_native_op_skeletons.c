@@ -8,6 +8,7 @@
  * DATAFLOW_NONE, and SHA-256 over the whole 388-byte header.
  */
 #include "set_native_op_skeletons.h"
+#include "set_native_score_op_skeletons.h"
 
 #include <ctype.h>
 #include <stdatomic.h>
@@ -22,7 +23,7 @@ typedef struct {
 	const char * name;
 	Nick_Form nick;
 	int num_args;
-	int args[12];
+	int args[16];
 	const char * init_symbol;
 } Native_Op_Spec;
 
@@ -65,6 +66,20 @@ static const Native_Op_Spec native_op_specs[] = {
 	 * 8 args, then values and copy_to_seq_context's context pointers and sizes */
 	{"rope_copy_to_seq_context", NICK_FWD, 11, {U64_S, I_S, I_S, I_S, I_S, DATAFLOW_INT, ARG_FWD, ARG_FWD, ARG_FWD,
 												 DATAFLOW_UINT64, DATAFLOW_INT}, NULL},
+	/* scoring ops, no reference counterpart: (rows, cols, row stride, scale,
+	 * tokens per row, top k, logits, tokens, logprobs, entropy, lse, top ids,
+	 * top logprobs, workspace bytes, workspace) */
+	{"token_logprobs",      NICK_FWD,    15, {I_S, I_S, U64_S, F_S, I_S, I_S, ARG_FWD, DATAFLOW_UINT32, DATAFLOW_FP32, DATAFLOW_FP32, DATAFLOW_FP32,
+											   DATAFLOW_UINT32, DATAFLOW_FP32, U64_S, DATAFLOW_VOID}, NULL},
+	/* (rows, cols, row stride, gradient stride, scale, tokens per row, logits,
+	 * tokens, lse, entropy, d logprobs, d entropy, d logits) */
+	{"token_logprobs_bwd",  NICK_FWD,    13, {I_S, I_S, U64_S, U64_S, F_S, I_S, ARG_FWD, DATAFLOW_UINT32, DATAFLOW_FP32, DATAFLOW_FP32,
+											   DATAFLOW_FP32, DATAFLOW_FP32, ARG_FWD}, NULL},
+	/* (rows, cols, row stride, gradient stride, scale, top k, logits, teacher
+	 * ids, teacher logits, row weights, loss, mean loss, d logits, workspace
+	 * bytes, workspace) */
+	{"distillation_loss",   NICK_FWD,    15, {I_S, I_S, U64_S, U64_S, F_S, I_S, ARG_FWD, DATAFLOW_UINT32, DATAFLOW_FP32, DATAFLOW_FP32,
+											   DATAFLOW_FP32, DATAFLOW_FP32, ARG_FWD, U64_S, DATAFLOW_VOID}, NULL},
 };
 
 #define NUM_NATIVE_OP_SPECS ((int) (sizeof(native_op_specs) / sizeof(native_op_specs[0])))
@@ -168,6 +183,9 @@ DEFINE_FWD_BWD_SETTER(set_native_softmax_skeleton, "softmax")
 DEFINE_BWD_SETTER(set_native_cross_entropy_loss_skeleton, "cross_entropy_loss")
 DEFINE_FWD_SETTER(set_native_softmax_cross_entropy_loss_skeleton, "softmax_cross_entropy_loss")
 DEFINE_FWD_SETTER(set_native_rope_copy_to_seq_context_skeleton, "rope_copy_to_seq_context")
+DEFINE_FWD_SETTER(set_native_token_logprobs_skeleton, "token_logprobs")
+DEFINE_FWD_SETTER(set_native_token_logprobs_bwd_skeleton, "token_logprobs_bwd")
+DEFINE_FWD_SETTER(set_native_distillation_loss_skeleton, "distillation_loss")
 
 /* ---- registration ---- */
 
@@ -206,7 +224,15 @@ static const Native_Variant native_variants[] = {
 	FWD3("rope_copy_to_seq_context"),
 };
 
+/* the scoring ops, a code object of their own */
+static const Native_Variant score_variants[] = {
+	FWD3("token_logprobs"),
+	FWD3("token_logprobs_bwd"),
+	FWD3("distillation_loss"),
+};
+
 #define NUM_NATIVE_VARIANTS ((int) (sizeof(native_variants) / sizeof(native_variants[0])))
+#define NUM_SCORE_VARIANTS ((int) (sizeof(score_variants) / sizeof(score_variants[0])))
 
 static void append_lower_dt(char * dst, size_t cap, DataflowDatatype dt) {
 	const char * s = dataflow_datatype_as_string(dt);
@@ -216,27 +242,27 @@ static void append_lower_dt(char * dst, size_t cap, DataflowDatatype dt) {
 	dst[len] = '\0';
 }
 
-int register_native_ops(Dataflow_Handle * dataflow_handle, char * native_function_code_filename, char * native_function_config_filename) {
-	int n = NUM_NATIVE_VARIANTS;
+static int register_variants(Dataflow_Handle * dataflow_handle, char * native_function_code_filename, char * native_function_config_filename,
+							 const Native_Variant * variants, int n, const char * what) {
 	Op_Skeleton * skeletons = (Op_Skeleton *) calloc((size_t) n, sizeof(Op_Skeleton));
 	char ** func_symbols = (char **) calloc((size_t) n, sizeof(char *));
 	char ** launch_symbols = (char **) calloc((size_t) n, sizeof(char *));
 	char ** init_symbols = (char **) calloc((size_t) n, sizeof(char *));
 	int added = -1;
 	if (!skeletons || !func_symbols || !launch_symbols || !init_symbols) {
-		fprintf(stderr, "Error: failed to allocate native op registration metadata...\n");
+		fprintf(stderr, "Error: failed to allocate %s op registration metadata...\n", what);
 		goto cleanup;
 	}
 
 	for (int i = 0; i < n; i++) {
-		const Native_Variant * v = &native_variants[i];
+		const Native_Variant * v = &variants[i];
 		const Native_Op_Spec * spec = find_spec(v->op);
 		build_skeleton(&skeletons[i], spec, v->fwd, v->bwd);
 
 		func_symbols[i] = (char *) calloc(FUNC_SYMBOL_MAX_LEN, 1);
 		launch_symbols[i] = (char *) calloc(FUNC_SYMBOL_MAX_LEN, 1);
 		if (!func_symbols[i] || !launch_symbols[i]) {
-			fprintf(stderr, "Error: failed to allocate native op symbol names...\n");
+			fprintf(stderr, "Error: failed to allocate %s op symbol names...\n", what);
 			goto cleanup;
 		}
 		snprintf(func_symbols[i], FUNC_SYMBOL_MAX_LEN, "%s", v->op);
@@ -254,7 +280,7 @@ int register_native_ops(Dataflow_Handle * dataflow_handle, char * native_functio
 	added = dataflow_handle->register_native_code(dataflow_handle, native_function_code_filename, native_function_config_filename,
 													n, skeletons, func_symbols, launch_symbols, init_symbols);
 	if (added != n) {
-		fprintf(stderr, "WARNING: failed to register all native ops, expected %d functions, got %d...\n", n, added);
+		fprintf(stderr, "WARNING: failed to register all %s ops, expected %d functions, got %d...\n", what, n, added);
 	}
 
 cleanup:
@@ -268,4 +294,14 @@ cleanup:
 	free(init_symbols);
 	free(skeletons);
 	return added;
+}
+
+int register_native_ops(Dataflow_Handle * dataflow_handle, char * native_function_code_filename, char * native_function_config_filename) {
+	return register_variants(dataflow_handle, native_function_code_filename, native_function_config_filename,
+							 native_variants, NUM_NATIVE_VARIANTS, "native");
+}
+
+int register_native_score_ops(Dataflow_Handle * dataflow_handle, char * score_function_code_filename, char * native_function_config_filename) {
+	return register_variants(dataflow_handle, score_function_code_filename, native_function_config_filename,
+							 score_variants, NUM_SCORE_VARIANTS, "scoring");
 }

@@ -1,0 +1,86 @@
+/*
+ * token_logprobs_bwd: the logits' gradient from those of the log-probabilities
+ * and of the entropy (formula in dataflow_score_ops.h). With G = sum_m g_m over
+ * the tokens that are columns, h the entropy's gradient and H the entropy,
+ *   dx_j = -s p_j (G + h (log p_j + H)) + s sum_m g_m [t_m = j].
+ * Every column gets the first term; the tokens' columns, whose logits are set
+ * aside before the first store (the gradient may lie in the logits' place),
+ * are then stored once more, whole, so that they are rounded once.
+ */
+#include "score_rows.h"
+
+struct GradTokens {
+	uint32_t id[SCORE_TOKENS_MAX];
+	float g[SCORE_TOKENS_MAX], x[SCORE_TOKENS_MAX];
+};
+
+/* s p (G + h (log p + H)) of a column */
+struct GradTerm {
+	float s, lse, down, h, H;
+	__device__ __forceinline__ float operator()(float x) const {
+		const float lp = fmaf(s, x, -lse);
+		const float p = __builtin_amdgcn_exp2f(lp * SCORE_LOG2E);
+		/* h = 0 drops the entropy's term also where log p is -inf */
+		const float f = h != 0.0f ? fmaf(h, fmaxf(lp, -1e30f) + H, down) : down;
+		return -s * p * f;
+	}
+};
+
+template <typename T>
+__device__ __forceinline__ void token_logprobs_bwd_run(int n_rows, int n_cols, uint64_t row_stride, uint64_t grad_stride, float s,
+													   int tokens_per_row, const T * logits, const uint32_t * tokens, const float * lse,
+													   const float * entropy, const float * d_logprobs, const float * d_entropy, T * dlogits) {
+	__shared__ float cells[SCORE_MAX_WAVES];
+	__shared__ GradTokens tok;
+	for (long r = blockIdx.x; r < n_rows; r += gridDim.x) {
+		const T * row = logits + (uint64_t) r * row_stride;
+		T * out = dlogits + (uint64_t) r * grad_stride;
+		__syncthreads();
+		float down = 0.0f, any = 0.0f;
+		for (int m = (int) threadIdx.x; m < tokens_per_row; m += (int) blockDim.x) {
+			const uint32_t t = tokens[r * tokens_per_row + m];
+			const bool is = t < (uint32_t) n_cols;
+			const float g = is ? d_logprobs[r * tokens_per_row + m] : 0.0f;
+			tok.id[m] = is ? t : 0xffffffffu;
+			tok.g[m] = g;
+			tok.x[m] = is ? to_f(row[t]) : 0.0f;
+			down += g;
+			any = g != 0.0f ? 1.0f : any;
+		}
+		down = score_group_sum(down, cells);
+		any = score_group_max(any, cells);
+		GradTerm term = {s, lse[r], down, d_entropy ? d_entropy[r] : 0.0f, d_entropy ? entropy[r] : 0.0f};
+		if ((any == 0.0f && term.h == 0.0f) || term.lse == -__builtin_inff()) {
+			for (long j = threadIdx.x; j < n_cols; j += blockDim.x) out[j] = from_f<T>(0.0f);
+			continue;
+		}
+		for (long j = threadIdx.x; j < n_cols; j += blockDim.x) out[j] = from_f<T>(term(to_f(row[j])));
+		__threadfence_block();
+		__builtin_amdgcn_s_waitcnt(0);
+		__syncthreads();
+		for (int m = (int) threadIdx.x; m < tokens_per_row; m += (int) blockDim.x) {
+			const uint32_t t = tok.id[m];
+			if (t == 0xffffffffu) continue;
+			float g = 0.0f;
+			bool first = true;
+			for (int o = 0; o < tokens_per_row; o++)
+				if (tok.id[o] == t) {
+					first = first && o >= m;
+					g += tok.g[o];
+				}
+			if (first) out[t] = from_f<T>(fmaf(s, g, term(tok.x[m])));
+		}
+	}
+}
+
+#define TOKEN_LOGPROBS_BWD_KERNEL(SUF, T)                                                                                      \
+	extern "C" __global__ void __launch_bounds__(SCORE_THREADS) token_logprobs_bwd_##SUF##_kernel(int n_rows, int n_cols,      \
+			uint64_t row_stride, uint64_t grad_stride, float scale, int tokens_per_row, T * logits, uint32_t * tokens,         \
+			float * lse, float * entropy, float * d_logprobs, float * d_entropy, T * dlogits) {                                \
+		token_logprobs_bwd_run<T>(n_rows, n_cols, row_stride, grad_stride, scale, tokens_per_row, logits, tokens, lse,         \
+								  entropy, d_logprobs, d_entropy, dlogits);                                                    \
+	}
+
+TOKEN_LOGPROBS_BWD_KERNEL(fp32, float)
+TOKEN_LOGPROBS_BWD_KERNEL(fp16, f16_t)
+TOKEN_LOGPROBS_BWD_KERNEL(bf16, bf16_t)

@@ -47,6 +47,12 @@ int softmax_cross_entropy_loss_set_launch_config(Hip_Launch_Config * hip_launch_
  * launch-wide state in the code object (shares_module_scratch) */
 int softmax_set_attribute_config(Dataflow_Handle * dataflow_handle, Hip_Function * hip_function);
 
+/* scoring ops (no reference counterpart) */
+int token_logprobs_set_launch_config(Hip_Launch_Config * hip_launch_config, Dataflow_Handle * dataflow_handle, Hip_Function * hip_function, Op * op);
+int token_logprobs_bwd_set_launch_config(Hip_Launch_Config * hip_launch_config, Dataflow_Handle * dataflow_handle, Hip_Function * hip_function, Op * op);
+int distillation_loss_set_launch_config(Hip_Launch_Config * hip_launch_config, Dataflow_Handle * dataflow_handle, Hip_Function * hip_function, Op * op);
+int distillation_loss_set_finish_launch_config(Hip_Launch_Config * hip_launch_config, Dataflow_Handle * dataflow_handle, Hip_Function * hip_function, Op * op);
+
 #ifdef __cplusplus
 }
 #endif

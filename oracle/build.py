@@ -1,7 +1,7 @@
 """Build recipe for the test oracle (TEST INFRASTRUCTURE ONLY).
 
-  oracle/liboracle.so    the C restatement (oracle.c) plus the CPU test backend
-                         (cpu_backend.c), linked against the product's libdataflow.so
+  oracle/liboracle.so    the C restatement (oracle.c), the scoring ops' oracle
+                         (score_ops.c) and the CPU test backend (cpu_backend.c), linked against the product's libdataflow.so
   oracle/libcpu_ref.so   the CPU baseline bench.py times (cpu_ref.c: fp32 math, fp64
                          reductions, OpenMP, AVX-512); built for x86-64-v4 rather
                          than -march=native, since it is compiled in this container
@@ -66,7 +66,7 @@ def build_oracle(verbose=False):
     tmp = ORACLE_OUT + ".tmp%d" % os.getpid()
     _run(["gcc", "-O2", "-fopenmp", "-fPIC", "-shared", "-std=gnu11", "-D__HIP_PLATFORM_AMD__",
           "-I", os.path.join(ROOT, "include"), "-I", HERE, "-I", "/opt/rocm/include",
-          os.path.join(HERE, "oracle.c"), os.path.join(HERE, "cpu_backend.c"),
+          os.path.join(HERE, "oracle.c"), os.path.join(HERE, "cpu_backend.c"), os.path.join(HERE, "score_ops.c"),
           "-o", tmp, "-L", PRODUCT_LIB, "-ldataflow", "-Wl,-rpath," + PRODUCT_LIB, "-lm"], verbose)
     os.replace(tmp, ORACLE_OUT)
     return ORACLE_OUT

@@ -69,6 +69,15 @@ int oracle_embedding(int elem_bytes, int num_tokens, int embed_dim, const uint32
 int oracle_copy_to_seq_context(int elem_bytes, uint64_t N, int kv_dim, const void * keys, const void * values,
 					const int * seq_positions, const uint64_t * ctx_ptrs, const int * ctx_sizes);
 
+/* the scoring ops (dataflow_score_ops.h), by their definitions; dx is
+ * [n_rows x n_cols] without gaps, outputs that may be NULL there may be here */
+int oracle_token_logprobs(int dt, int n_rows, int n_cols, uint64_t row_stride, float scale, int tokens_per_row, int top_k, const void * logits,
+					const uint32_t * tokens, double * logprobs, double * entropy, double * lse, uint32_t * top_ids, double * top_logprobs);
+int oracle_token_logprobs_bwd(int dt, int n_rows, int n_cols, uint64_t row_stride, float scale, int tokens_per_row, const void * logits,
+					const uint32_t * tokens, const float * lse, const float * entropy, const float * d_logprobs, const float * d_entropy, double * dx);
+int oracle_distillation_loss(int dt, int n_rows, int n_cols, uint64_t row_stride, float scale, int top_k, const void * logits,
+					const uint32_t * teacher_ids, const float * teacher_logits, const float * row_weights, double * loss, double * mean_loss, double * dx);
+
 /* exact rounding chains (no evaluation slack) */
 int oracle_rms_norm_bwd_x_exact(int dt, int n_rows, int n_cols, const float * ws, const float * rs,
 					const void * W, const void * X, const void * dY, const void * dX_in, double * v);
