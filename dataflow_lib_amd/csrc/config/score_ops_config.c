@@ -10,14 +10,14 @@
 
 #define ARG(op, i, type) (*((type *) (op)->op_args[(i)]))
 
-static void set_1d(Hip_Launch_Config * c, unsigned grid, unsigned block) {
+static void set_1d(Hip_Launch_Config * c, unsigned grid, unsigned block, unsigned lds) {
 	c->gridDimX = grid;
 	c->gridDimY = 1;
 	c->gridDimZ = 1;
 	c->blockDimX = block;
 	c->blockDimY = 1;
 	c->blockDimZ = 1;
-	c->sharedMemBytes = 0;
+	c->sharedMemBytes = lds;
 }
 
 /* an operand that the kernels access: there, and aligned to its elements */
@@ -78,7 +78,7 @@ static size_t logits_elem(Hip_Function * f) { return dataflow_sizeof_element(f->
 
 /* one workgroup per row */
 static void rows_config(Hip_Launch_Config * c, int n_rows) {
-	set_1d(c, (unsigned) MY_MIN(n_rows, SCORE_MAX_GROUPS), SCORE_THREADS);
+	set_1d(c, (unsigned) MY_MIN(n_rows, SCORE_MAX_GROUPS), SCORE_THREADS, 0);
 }
 
 int token_logprobs_set_launch_config(Hip_Launch_Config * hip_launch_config, Dataflow_Handle * dataflow_handle, Hip_Function * hip_function, Op * op) {
@@ -94,7 +94,7 @@ int token_logprobs_set_launch_config(Hip_Launch_Config * hip_launch_config, Data
 	const int checked = score_check(what, n_rows, n_cols, ARG(op, 2, uint64_t), ARG(op, 3, float), ARG(op, 6, void *), elem);
 	if (checked < 0) return -1;
 	if (checked == 0) {
-		set_1d(hip_launch_config, 0, 1);
+		set_1d(hip_launch_config, 0, 1, 0);
 		return 0;
 	}
 	if (top_k > n_cols) {
@@ -108,9 +108,22 @@ int token_logprobs_set_launch_config(Hip_Launch_Config * hip_launch_config, Data
 	if (top_k > 0 && (score_pointer(what, "the top id pointer", ARG(op, 11, void *), 4) ||
 					  score_pointer(what, "the top log-probability pointer", ARG(op, 12, void *), 4))) return -1;
 	if (score_check_workspace(what, score_logprobs_workspace(n_rows, n_cols, (int) elem, top_k), ARG(op, 13, uint64_t), ARG(op, 14, void *))) return -1;
-	rows_config(hip_launch_config, n_rows);
+	const Score_Plan plan = score_stream_plan(n_rows, n_cols, (int) elem);
+	const long groups = (long) n_rows * plan.slices;
+	set_1d(hip_launch_config, (unsigned) MY_MIN(groups, (long) SCORE_MAX_GROUPS), (unsigned) (64 * plan.waves),
+		   top_k > 0 ? score_top_lds(plan.waves) : 0);
 	return 0;
 }
+
+/* rows of several slices: their join */
+int token_logprobs_set_finish_launch_config(Hip_Launch_Config * hip_launch_config, Dataflow_Handle * dataflow_handle, Hip_Function * hip_function, Op * op) {
+	(void) dataflow_handle;
+	const int n_rows = ARG(op, 0, int), top_k = ARG(op, 5, int);
+	const Score_Plan plan = score_stream_plan(n_rows, ARG(op, 1, int), (int) logits_elem(hip_function));
+	set_1d(hip_launch_config, plan.slices > 1 ? (unsigned) n_rows : 0u, SCORE_THREADS, (unsigned) (8 * plan.slices * top_k));
+	return 0;
+}
+
 
 int token_logprobs_bwd_set_launch_config(Hip_Launch_Config * hip_launch_config, Dataflow_Handle * dataflow_handle, Hip_Function * hip_function, Op * op) {
 	(void) dataflow_handle;
@@ -124,7 +137,7 @@ int token_logprobs_bwd_set_launch_config(Hip_Launch_Config * hip_launch_config, 
 	const int checked = score_check(what, n_rows, n_cols, ARG(op, 2, uint64_t), ARG(op, 4, float), ARG(op, 6, void *), elem);
 	if (checked < 0) return -1;
 	if (checked == 0) {
-		set_1d(hip_launch_config, 0, 1);
+		set_1d(hip_launch_config, 0, 1, 0);
 		return 0;
 	}
 	if (tokens_per_row > 0 && (score_pointer(what, "the token pointer", ARG(op, 7, void *), 4) ||
@@ -149,7 +162,7 @@ int distillation_loss_set_launch_config(Hip_Launch_Config * hip_launch_config, D
 	const int checked = score_check(what, n_rows, n_cols, ARG(op, 2, uint64_t), ARG(op, 4, float), ARG(op, 6, void *), elem);
 	if (checked < 0) return -1;
 	if (checked == 0) {
-		set_1d(hip_launch_config, 0, 1);
+		set_1d(hip_launch_config, 0, 1, 0);
 		return 0;
 	}
 	if (top_k > 0 && (score_pointer(what, "the teacher id pointer", ARG(op, 7, void *), 4) ||
@@ -167,6 +180,6 @@ int distillation_loss_set_launch_config(Hip_Launch_Config * hip_launch_config, D
 int distillation_loss_set_finish_launch_config(Hip_Launch_Config * hip_launch_config, Dataflow_Handle * dataflow_handle, Hip_Function * hip_function, Op * op) {
 	(void) dataflow_handle;
 	(void) hip_function;
-	set_1d(hip_launch_config, ARG(op, 11, void *) ? 1u : 0u, SCORE_THREADS);
+	set_1d(hip_launch_config, ARG(op, 11, void *) ? 1u : 0u, SCORE_THREADS, 0);
 	return 0;
 }

@@ -18,7 +18,7 @@ template <typename T>
 __device__ __forceinline__ void distillation_loss_run(int n_rows, int n_cols, uint64_t row_stride, uint64_t grad_stride, float s, int top_k,
 													  const T * logits, const uint32_t * teacher_ids, const float * teacher_logits,
 													  const float * row_weights, float * loss, T * dlogits) {
-	__shared__ float cells[SCORE_MAX_WAVES];
+	__shared__ float cells[3 * SCORE_MAX_WAVES];
 	__shared__ Teacher te;
 	const float temperature = 1.0f / s;
 	for (long r = blockIdx.x; r < n_rows; r += gridDim.x) {

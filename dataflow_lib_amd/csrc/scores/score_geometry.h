@@ -7,7 +7,11 @@
 #define SCORE_GEOMETRY_H
 
 #ifndef GEOM_FN
+#ifdef __HIPCC__
+#define GEOM_FN __host__ __device__ static inline
+#else
 #define GEOM_FN static inline
+#endif
 #endif
 
 /* limits of the public interface (dataflow_score_ops.h) */
@@ -17,19 +21,71 @@
 #define SCORE_SCALE_MIN 1e-6f
 #define SCORE_SCALE_MAX 1e6f
 
-/* one workgroup per row, walking rows a grid apart: so many workgroups at
- * most, which keeps every launch below 2^32 threads */
-#define SCORE_THREADS 256
+/* so many workgroups at most, which walk what is left: every launch stays
+ * below 2^32 threads */
 #define SCORE_MAX_GROUPS (1 << 20)
+/* simple row kernels and the mean loss */
+#define SCORE_THREADS 256
+
+/* Streaming kernels: a row is cut into slices of whole 16-byte chunks (the
+ * last one takes the elements behind the last whole chunk too), a workgroup
+ * per slice, whose threads take SCORE_BATCH chunks at a time. */
+#define SCORE_BATCH 8   /* twice what score_stream begins its rest with */
+#define SCORE_STREAM_WAVES 8
+/* few rows: slices until the chip has this many waves */
+#define SCORE_FILL_WAVES 2048
+#define SCORE_MAX_SLICES 32
+
+/* how a call's rows are cut */
+typedef struct {
+	int waves;          /* per workgroup */
+	int slices;         /* per row */
+	int slice_chunks;   /* per slice; the last may have fewer */
+} Score_Plan;
+
+GEOM_FN Score_Plan score_stream_plan(int n_rows, int n_cols, int elem_bytes) {
+	Score_Plan p;
+	const long chunks = (long) n_cols * elem_bytes / 16;
+	const long per_wave = 64 * SCORE_BATCH;
+	long waves = (chunks + per_wave - 1) / per_wave;   /* that the row fills with a batch each */
+	if (waves < 1) waves = 1;
+	p.waves = (int) (waves < SCORE_STREAM_WAVES ? waves : SCORE_STREAM_WAVES);
+	p.slices = 1;
+	/* a slice keeps every wave of its workgroup busy with a batch */
+	const long most = waves / SCORE_STREAM_WAVES;
+	long want = SCORE_FILL_WAVES / ((long) n_rows * p.waves);
+	if (want > most) want = most;
+	if (want > SCORE_MAX_SLICES) want = SCORE_MAX_SLICES;
+	if (want > 1) p.slices = (int) want;
+	p.slice_chunks = (int) ((chunks + p.slices - 1) / p.slices);
+	if (p.slices > 1) p.slices = (int) ((chunks + p.slice_chunks - 1) / p.slice_chunks);
+	return p;
+}
+
+/* what a slice of a row leaves in the workspace: its statistics, and its
+ * top_k alternatives, largest first */
+typedef struct {
+	float max, z, e, unused;
+} Score_Part;
 
 GEOM_FN unsigned long score_logprobs_workspace(int n_rows, int n_cols, int elem_bytes, int top_k) {
-	(void) n_rows; (void) n_cols; (void) elem_bytes; (void) top_k;
-	return 0;
+	if (n_rows <= 0 || n_cols <= 0 || elem_bytes <= 0 || top_k < 0) return 0;
+	const Score_Plan p = score_stream_plan(n_rows, n_cols, elem_bytes);
+	if (p.slices == 1) return 0;
+	return (unsigned long) n_rows * (unsigned long) p.slices * (sizeof(Score_Part) + 8ul * (unsigned long) top_k);
 }
 
 GEOM_FN unsigned long score_distill_workspace(int n_rows, int n_cols, int elem_bytes, int top_k) {
 	(void) n_rows; (void) n_cols; (void) elem_bytes; (void) top_k;
 	return 0;
+}
+
+/* token_logprobs: LDS of a workgroup with alternatives to find. Group maxima
+ * (SCORE_GROUP_SLOTS per thread) and candidates. */
+#define SCORE_GROUP_SLOTS 4
+#define SCORE_CANDIDATES 1024
+GEOM_FN unsigned score_top_lds(int waves) {
+	return (unsigned) (waves * 64 * SCORE_GROUP_SLOTS * 4 + SCORE_CANDIDATES * 8);
 }
 
 #endif

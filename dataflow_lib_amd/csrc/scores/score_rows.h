@@ -1,12 +1,18 @@
 /*
- * What the scoring kernels share: a row's statistics and its k largest
- * logits, each found by one workgroup.
+ * What the scoring kernels share: a row's statistics in one pass over its
+ * logits, and its k largest logits.
  *
  * A row is shifted by its largest logit M before anything is exponentiated:
  *   Z = sum exp(s (x - M)),  E = sum s (x - M) exp(s (x - M))
  *   lse = s M + log Z,  log p_j = s (x_j - M) - log Z,  entropy = log Z - E / Z
  * The difference x - M is formed first: it is exact next to the maximum, and
- * it cannot overflow where s x can (rows of the type's lowest value).
+ * it cannot overflow where s x can (rows of the type's lowest value). In one
+ * pass every thread shifts by the largest logit that it has met so far and
+ * moves its sums when that grows, from a to b:
+ *   Z <- f Z,  E <- f (E + s (a - b) Z),  f = exp(s (a - b))
+ * where all terms of E have one sign, so nothing cancels; threads, waves and
+ * slices are joined in the same way, in a fixed order. Exponents are in units
+ * of log 2 (t = s log2(e) (x - M)), and so is E until the end.
  */
 #pragma once
 
@@ -15,21 +21,25 @@
 #include "score_geometry.h"
 
 #define SCORE_LOG2E 1.4426950408889634f
+#define SCORE_LN2 0.6931471805599453f
 #define SCORE_MAX_WAVES 16
+/* exp2 of it is 0; finite, so that it times 0 is 0 */
+#define SCORE_FAR_BELOW -1e4f
 
 /* what a row's log-probabilities are formed from */
 struct RowStats {
-	float max;      /* M; 0 for a row of -inf alone */
+	float max;      /* M */
 	float log_z;    /* log Z; +inf for a row of -inf alone, NaN with NaN or +inf */
 	float inv_z;    /* 1 / Z; 0 for a row of -inf alone */
 	float e_z;      /* E / Z */
 	__device__ __forceinline__ RowStats() {}
+	/* e in units of log 2 */
 	__device__ __forceinline__ RowStats(float m, float z, float e) {
-		max = m;
 		const bool none = z == 0.0f;
+		max = none ? 0.0f : m;
 		log_z = none ? __builtin_inff() : logf(z);
 		inv_z = none ? 0.0f : 1.0f / z;
-		e_z = none ? 0.0f : e / z;
+		e_z = none ? 0.0f : e / z * SCORE_LN2;
 	}
 	__device__ __forceinline__ bool none() const { return inv_z == 0.0f; }
 	__device__ __forceinline__ float lse(float s) const { return none() ? -__builtin_inff() : fmaf(s, max, log_z); }
@@ -37,13 +47,20 @@ struct RowStats {
 	__device__ __forceinline__ float log_p(float x, float s) const { return s * (x - max) - log_z; }
 };
 
-/* a term of Z (into z) and of E (into e): t = s (x - M) in units of log2, and a
- * column of -inf counts nothing (-inf * 0 is kept out of E) */
-__device__ __forceinline__ void score_add(float d, float s_log2e, float s, float & z, float & e) {
-	const float p = __builtin_amdgcn_exp2f(d * s_log2e);
-	z += p;
-	e = fmaf(fmaxf(d, -1e30f) * s, p, e);
-}
+/* maximum and sums of a part of a row */
+struct RowPart {
+	float m, z, e;
+	__device__ __forceinline__ RowPart() { m = -__builtin_inff(); z = 0.0f; e = 0.0f; }
+	/* shifted by a larger maximum. Maxima that differ by infinity or are both
+	 * -inf (NaN) give the far-below shift, whose sums are 0. */
+	__device__ __forceinline__ void shift(float to, float s_log2e) {
+		const float t = fmaxf((m - to) * s_log2e, SCORE_FAR_BELOW);
+		const float f = __builtin_amdgcn_exp2f(t);
+		e = f * fmaf(t, z, e);
+		z = f * z;
+		m = to;
+	}
+};
 
 /* sums and maxima over a workgroup; `cells`: SCORE_MAX_WAVES floats of LDS */
 __device__ __forceinline__ float score_group_max(float v, float * cells) {
@@ -66,18 +83,172 @@ __device__ __forceinline__ float score_group_sum(float v, float * cells) {
 	for (int w = 1; w < waves; w++) v += cells[w];
 	return v;
 }
+/* the parts of a workgroup's threads, joined (every thread gets the result);
+ * `cells`: 3 SCORE_MAX_WAVES floats of LDS */
+__device__ __forceinline__ RowPart score_group_join(RowPart p, float s_log2e, float * cells) {
+	const int wave = (int) (threadIdx.x >> 6), waves = (int) (blockDim.x >> 6);
+	p.shift(wave_max(p.m), s_log2e);
+	p.z = wave_sum(p.z);
+	p.e = wave_sum(p.e);
+	if (waves == 1) return p;
+	__syncthreads();
+	if ((threadIdx.x & 63) == 0) {
+		cells[wave] = p.m;
+		cells[SCORE_MAX_WAVES + wave] = p.z;
+		cells[2 * SCORE_MAX_WAVES + wave] = p.e;
+	}
+	__syncthreads();
+	float m = cells[0];
+	for (int w = 1; w < waves; w++) m = fmaxf(m, cells[w]);
+	RowPart sum;
+	sum.m = m;
+	for (int w = 0; w < waves; w++) {
+		RowPart q;
+		q.m = cells[w];
+		q.z = cells[SCORE_MAX_WAVES + w];
+		q.e = cells[2 * SCORE_MAX_WAVES + w];
+		q.shift(m, s_log2e);
+		sum.z += q.z;
+		sum.e += q.e;
+	}
+	return sum;
+}
+
+/* 16 bytes of a row, which need no more alignment than its elements (of two
+ * bytes at least) */
+typedef uint32_t score_vec __attribute__((ext_vector_type(4), aligned(2)));
+template <typename T>
+__device__ __forceinline__ R16 score_load(const T * row, uint64_t uniform_chunk, uint32_t lane_chunk) {
+	const char * p = reinterpret_cast<const char *>(row) + uniform_chunk * 16u;
+	const score_vec v = __builtin_nontemporal_load(reinterpret_cast<const score_vec *>(p + lane_chunk * 16u));
+	R16 r;
+	r.w[0] = v.x; r.w[1] = v.y; r.w[2] = v.z; r.w[3] = v.w;
+	return r;
+}
+
+/* the elements of a row that a workgroup works on: chunks [first, last), and
+ * for the last slice the elements from `tail` to the row's end */
+struct RowSlice {
+	int first, last, tail, end;
+	__device__ __forceinline__ RowSlice(int n_cols, int vec, int slice, int slices, int slice_chunks) {
+		const int chunks = n_cols / vec;
+		first = slice * slice_chunks;
+		last = slice + 1 == slices ? chunks : first + slice_chunks;
+		tail = slice + 1 == slices ? chunks * vec : n_cols;
+		end = n_cols;
+	}
+	__device__ __forceinline__ long columns(int vec) const { return (long) (last - first) * vec + (end - tail); }
+};
+
+/* N chunks (c + tid, a workgroup's threads apart) into a thread's part: their
+ * maximum, the part's shift to it, then their terms. -inf makes E's term NaN
+ * (-inf * 0): a wave that finds NaN in its sum forms the terms again, with
+ * exponents that are far below 0 but finite. Returns the chunks' maximum. */
+template <typename T, int N, bool ENTROPY>
+__device__ __forceinline__ float score_chunks(const T * row, int c, float s_log2e, RowPart & p) {
+	constexpr int V = VecOf<T>::N;
+	R16 x[N];
+#pragma unroll
+	for (int u = 0; u < N; u++) x[u] = score_load(row, (uint64_t) (c + u * (int) blockDim.x), threadIdx.x);
+	float m = -__builtin_inff();
+#pragma unroll
+	for (int u = 0; u < N; u++) {
+		float f[V];
+		unpack16<T>(x[u], f);
+#pragma unroll
+		for (int i = 0; i < V; i++) m = fmaxf(m, f[i]);
+	}
+	p.shift(fmaxf(p.m, m), s_log2e);
+	/* a thread that has met -inf alone keeps its differences from being NaN */
+	const float ref = p.m == -__builtin_inff() ? 0.0f : p.m;
+	float z[2] = {0.0f, 0.0f}, e[2] = {0.0f, 0.0f};
+#pragma unroll
+	for (int u = 0; u < N; u++) {
+		/* a chunk at a time: left to itself the compiler keeps all chunks' terms
+		 * at once, at twice the registers */
+		__builtin_amdgcn_sched_barrier(0);
+		reg_barrier(x[u]);
+		float f[V];
+		unpack16<T>(x[u], f);
+#pragma unroll
+		for (int i = 0; i < V; i++) {
+			const float t = (f[i] - ref) * s_log2e;
+			const float q = __builtin_amdgcn_exp2f(t);
+			z[i & 1] += q;
+			if (ENTROPY) e[i & 1] = fmaf(t, q, e[i & 1]);
+		}
+	}
+	float eb = e[0] + e[1], zb = z[0] + z[1];
+	/* or the sum of z is moved behind the branch, and all its terms are kept */
+	__asm__ volatile("" : "+v"(zb));
+	if (ENTROPY && __builtin_expect(__any(eb != eb), 0)) {
+		eb = 0.0f;
+#pragma unroll
+		for (int u = 0; u < N; u++) {
+			__builtin_amdgcn_sched_barrier(0);
+			reg_barrier(x[u]);
+			float f[V];
+			unpack16<T>(x[u], f);
+#pragma unroll
+			for (int i = 0; i < V; i++) {
+				const float t = fmaxf((f[i] - ref) * s_log2e, SCORE_FAR_BELOW);
+				eb = fmaf(t, __builtin_amdgcn_exp2f(t), eb);
+			}
+		}
+	}
+	p.z += zb;
+	p.e += eb;
+	return m;
+}
+
+/* A thread's part of a slice: batches of SCORE_BATCH chunks, and what is left
+ * in batches of half, a quarter and so on, so that only the last chunk has to
+ * ask whether it is there. The maximum of the thread's b-th batch (what is left
+ * being one) goes to groups[(b % SCORE_GROUP_SLOTS) * blockDim.x + tid] (LDS;
+ * null: not wanted); the element behind the last whole chunk counts to batch 0. */
+template <typename T, bool ENTROPY>
+__device__ __forceinline__ RowPart score_stream(const T * row, const RowSlice & sl, float s_log2e, float * groups) {
+	const int nt = (int) blockDim.x, tid = (int) threadIdx.x;
+	RowPart p;
+	float before = -__builtin_inff();
+	if (sl.tail + tid < sl.end) {
+		const float x = to_f(row[sl.tail + tid]);
+		p.m = before = fmaxf(x, -__builtin_inff());   /* NaN: -inf */
+		p.z = __builtin_amdgcn_exp2f((x - (p.m == -__builtin_inff() ? 0.0f : p.m)) * s_log2e);
+	}
+	int slot = 0;
+	bool again = false;
+	for (int c = sl.first;;) {
+		float m;
+		const bool whole = c + SCORE_BATCH * nt <= sl.last;
+		if (whole) {
+			m = score_chunks<T, SCORE_BATCH, ENTROPY>(row, c, s_log2e, p);
+			c += SCORE_BATCH * nt;
+		}
+		else {
+			m = -__builtin_inff();
+			if (c + 4 * nt <= sl.last) { m = fmaxf(m, score_chunks<T, 4, ENTROPY>(row, c, s_log2e, p)); c += 4 * nt; }
+			if (c + 2 * nt <= sl.last) { m = fmaxf(m, score_chunks<T, 2, ENTROPY>(row, c, s_log2e, p)); c += 2 * nt; }
+			if (c + nt <= sl.last) { m = fmaxf(m, score_chunks<T, 1, ENTROPY>(row, c, s_log2e, p)); c += nt; }
+			if (c + tid < sl.last) m = fmaxf(m, score_chunks<T, 1, ENTROPY>(row, c, s_log2e, p));
+		}
+		if (groups) {
+			float * g = groups + slot * nt + tid;
+			*g = fmaxf(m, again ? *g : before);
+			before = -__builtin_inff();
+		}
+		if (!whole || c >= sl.last) break;
+		if (++slot == SCORE_GROUP_SLOTS) { slot = 0; again = true; }
+	}
+	return p;
+}
 
 template <typename T>
 __device__ __forceinline__ RowStats score_row_stats(const T * row, int n_cols, float s, float * cells) {
-	float m = -__builtin_inff();
-	for (long j = threadIdx.x; j < n_cols; j += blockDim.x) m = fmaxf(m, to_f(row[j]));
-	m = score_group_max(m, cells);
-	if (m == -__builtin_inff()) m = 0.0f;
-	float z = 0.0f, e = 0.0f;
-	for (long j = threadIdx.x; j < n_cols; j += blockDim.x) score_add(to_f(row[j]) - m, s * SCORE_LOG2E, s, z, e);
-	z = score_group_sum(z, cells);
-	e = score_group_sum(e, cells);
-	return RowStats(m, z, e);
+	constexpr int V = VecOf<T>::N;
+	const RowSlice sl(n_cols, V, 0, 1, n_cols / V);
+	const RowPart p = score_group_join(score_stream<T, false>(row, sl, s * SCORE_LOG2E, nullptr), s * SCORE_LOG2E, cells);
+	return RowStats(p.m, p.z, p.e);
 }
 
 /* Whole numbers that lie as floats do: -0 with +0, NaN below -inf. */
@@ -86,77 +257,12 @@ __device__ __forceinline__ uint32_t score_key(float x) {
 	if (x != x) return 0u;
 	return (u >> 31) ? ~u : (u | 0x80000000u);
 }
-
-/* A row's k largest logits, found exactly: the k-th largest key digit by digit
- * (8 bits of it a pass over the row, counted in LDS), then the larger ones and
- * as many of the equal ones, by rising column, as are left. */
-struct ScoreTop {
-	uint32_t hist[256];
-	uint32_t prefix, need, count;
-	uint32_t waves[SCORE_MAX_WAVES];
-	uint32_t key[SCORE_TOP_MAX], id[SCORE_TOP_MAX];
-};
-
-template <typename T>
-__device__ __forceinline__ void score_select(const T * row, int n_cols, int k, ScoreTop & t) {
-	const int tid = (int) threadIdx.x, lane = tid & 63, wave = tid >> 6, n_waves = (int) (blockDim.x >> 6);
-	__syncthreads();
-	if (tid == 0) { t.prefix = 0u; t.need = (uint32_t) k; t.count = 0u; }
-	for (int shift = 24; shift >= 0; shift -= 8) {
-		for (int b = tid; b < 256; b += (int) blockDim.x) t.hist[b] = 0u;
-		__syncthreads();
-		const uint32_t prefix = t.prefix;
-		const uint32_t above = shift == 24 ? 0u : 0xffffffffu << (shift + 8);
-		for (long j = tid; j < n_cols; j += blockDim.x) {
-			const uint32_t key = score_key(to_f(row[j]));
-			if ((key & above) == prefix) atomicAdd(&t.hist[(key >> shift) & 255u], 1u);
-		}
-		__syncthreads();
-		if (tid == 0) {
-			uint32_t need = t.need;
-			int b = 255;
-			while (b > 0 && t.hist[b] < need) need -= t.hist[b--];
-			t.prefix = prefix | ((uint32_t) b << shift);
-			t.need = need;
-		}
-		__syncthreads();
-	}
-	const uint32_t last = t.prefix, equal = t.need;
-	for (long j = tid; j < n_cols; j += blockDim.x) {
-		const uint32_t key = score_key(to_f(row[j]));
-		if (key > last) {
-			const uint32_t at = atomicAdd(&t.count, 1u);
-			t.key[at] = key;
-			t.id[at] = (uint32_t) j;
-		}
-	}
-	/* the equal ones in the order of their columns */
-	uint32_t have = 0;
-	for (long base = 0; base < n_cols && have < equal; base += blockDim.x) {
-		const long j = base + tid;
-		const bool is = j < n_cols && score_key(to_f(row[j < n_cols ? j : 0])) == last;
-		const unsigned long long ballot = __ballot(is);
-		__syncthreads();
-		if (lane == 0) t.waves[wave] = (uint32_t) __popcll(ballot);
-		__syncthreads();
-		uint32_t before = have + (uint32_t) __popcll(ballot & ((1ull << lane) - 1ull));
-		for (int w = 0; w < n_waves; w++) {
-			if (w < wave) before += t.waves[w];
-			have += t.waves[w];
-		}
-		if (is && before < equal) {
-			t.key[(uint32_t) k - equal + before] = last;
-			t.id[(uint32_t) k - equal + before] = (uint32_t) j;
-		}
-	}
-	__syncthreads();
+__device__ __forceinline__ float score_key_value(uint32_t key) {
+	if (key == 0u) return __builtin_nanf("");
+	return __uint_as_float((key >> 31) ? key & 0x7fffffffu : ~key);
 }
-
-/* the place of each chosen logit among the k: by falling key, equal keys by
- * rising column */
-__device__ __forceinline__ int score_rank(const ScoreTop & t, int k, int i) {
-	const uint32_t key = t.key[i], id = t.id[i];
-	int r = 0;
-	for (int o = 0; o < k; o++) r += (t.key[o] > key || (t.key[o] == key && t.id[o] < id)) ? 1 : 0;
-	return r;
-}
+/* An alternative as one number: larger logits are larger numbers, and of equal
+ * ones the lower column's; 0 is none. */
+__device__ __forceinline__ uint64_t score_alternative(uint32_t key, uint32_t id) { return ((uint64_t) key << 32) | (0xffffffffu - id); }
+__device__ __forceinline__ uint32_t score_alternative_id(uint64_t a) { return 0xffffffffu - (uint32_t) a; }
+__device__ __forceinline__ float score_alternative_value(uint64_t a) { return score_key_value((uint32_t) (a >> 32)); }
