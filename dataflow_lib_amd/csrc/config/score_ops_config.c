@@ -76,6 +76,11 @@ static int score_check_workspace(const char * what, uint64_t needed, uint64_t by
 
 static size_t logits_elem(Hip_Function * f) { return dataflow_sizeof_element(f->op_skeleton.header.arg_dtypes[6]); }
 
+/* a workgroup per slice */
+static void plan_config(Hip_Launch_Config * c, Score_Plan plan, int n_rows, unsigned lds) {
+	set_1d(c, (unsigned) MY_MIN((long) n_rows * plan.slices, (long) SCORE_MAX_GROUPS), (unsigned) (64 * plan.waves), lds);
+}
+
 /* one workgroup per row */
 static void rows_config(Hip_Launch_Config * c, int n_rows) {
 	set_1d(c, (unsigned) MY_MIN(n_rows, SCORE_MAX_GROUPS), SCORE_THREADS, 0);
@@ -109,9 +114,7 @@ int token_logprobs_set_launch_config(Hip_Launch_Config * hip_launch_config, Data
 					  score_pointer(what, "the top log-probability pointer", ARG(op, 12, void *), 4))) return -1;
 	if (score_check_workspace(what, score_logprobs_workspace(n_rows, n_cols, (int) elem, top_k), ARG(op, 13, uint64_t), ARG(op, 14, void *))) return -1;
 	const Score_Plan plan = score_stream_plan(n_rows, n_cols, (int) elem);
-	const long groups = (long) n_rows * plan.slices;
-	set_1d(hip_launch_config, (unsigned) MY_MIN(groups, (long) SCORE_MAX_GROUPS), (unsigned) (64 * plan.waves),
-		   top_k > 0 ? score_top_lds(plan.waves) : 0);
+	plan_config(hip_launch_config, plan, n_rows, top_k > 0 ? score_top_lds(plan.waves) : 0);
 	return 0;
 }
 
@@ -146,7 +149,7 @@ int token_logprobs_bwd_set_launch_config(Hip_Launch_Config * hip_launch_config, 
 	if (ARG(op, 11, void *) && (score_pointer(what, "the entropy gradient pointer", ARG(op, 11, void *), 4) ||
 								score_pointer(what, "the entropy pointer", ARG(op, 9, void *), 4))) return -1;
 	if (score_check_grad(what, n_rows, n_cols, ARG(op, 2, uint64_t), ARG(op, 3, uint64_t), ARG(op, 6, void *), ARG(op, 12, void *), elem)) return -1;
-	rows_config(hip_launch_config, n_rows);
+	plan_config(hip_launch_config, score_map_plan(n_rows, n_cols, (int) elem), n_rows, 0);
 	return 0;
 }
 

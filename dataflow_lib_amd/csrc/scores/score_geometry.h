@@ -32,6 +32,7 @@
  * per slice, whose threads take SCORE_BATCH chunks at a time. */
 #define SCORE_BATCH 8   /* twice what score_stream begins its rest with */
 #define SCORE_STREAM_WAVES 8
+#define SCORE_MAP_BATCH 2
 /* few rows: slices until the chip has this many waves */
 #define SCORE_FILL_WAVES 2048
 #define SCORE_MAX_SLICES 32
@@ -43,16 +44,18 @@ typedef struct {
 	int slice_chunks;   /* per slice; the last may have fewer */
 } Score_Plan;
 
-GEOM_FN Score_Plan score_stream_plan(int n_rows, int n_cols, int elem_bytes) {
+/* waves that a row fills with `batch` chunks per thread, at most max_waves of
+ * them to a workgroup; few rows are cut into slices of whole such workgroups
+ * until the chip has SCORE_FILL_WAVES waves */
+GEOM_FN Score_Plan score_plan(int n_rows, int n_cols, int elem_bytes, int batch, int max_waves) {
 	Score_Plan p;
 	const long chunks = (long) n_cols * elem_bytes / 16;
-	const long per_wave = 64 * SCORE_BATCH;
-	long waves = (chunks + per_wave - 1) / per_wave;   /* that the row fills with a batch each */
+	const long per_wave = 64 * batch;
+	long waves = (chunks + per_wave - 1) / per_wave;
 	if (waves < 1) waves = 1;
-	p.waves = (int) (waves < SCORE_STREAM_WAVES ? waves : SCORE_STREAM_WAVES);
+	p.waves = (int) (waves < max_waves ? waves : max_waves);
 	p.slices = 1;
-	/* a slice keeps every wave of its workgroup busy with a batch */
-	const long most = waves / SCORE_STREAM_WAVES;
+	const long most = waves / max_waves;
 	long want = SCORE_FILL_WAVES / ((long) n_rows * p.waves);
 	if (want > most) want = most;
 	if (want > SCORE_MAX_SLICES) want = SCORE_MAX_SLICES;
@@ -60,6 +63,16 @@ GEOM_FN Score_Plan score_stream_plan(int n_rows, int n_cols, int elem_bytes) {
 	p.slice_chunks = (int) ((chunks + p.slices - 1) / p.slices);
 	if (p.slices > 1) p.slices = (int) ((chunks + p.slice_chunks - 1) / p.slice_chunks);
 	return p;
+}
+
+GEOM_FN Score_Plan score_stream_plan(int n_rows, int n_cols, int elem_bytes) {
+	return score_plan(n_rows, n_cols, elem_bytes, SCORE_BATCH, SCORE_STREAM_WAVES);
+}
+
+/* the gradient kernels, which read and write a row once */
+#define SCORE_MAP_WAVES 8
+GEOM_FN Score_Plan score_map_plan(int n_rows, int n_cols, int elem_bytes) {
+	return score_plan(n_rows, n_cols, elem_bytes, SCORE_MAP_BATCH, SCORE_MAP_WAVES);
 }
 
 /* what a slice of a row leaves in the workspace: its statistics, and its

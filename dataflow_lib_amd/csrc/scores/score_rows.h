@@ -137,6 +137,9 @@ struct RowSlice {
 		tail = slice + 1 == slices ? chunks * vec : n_cols;
 		end = n_cols;
 	}
+	__device__ __forceinline__ bool holds(uint32_t column, int vec) const {
+		return column >= (uint32_t) first * (uint32_t) vec && (column < (uint32_t) last * (uint32_t) vec || column >= (uint32_t) tail) && column < (uint32_t) end;
+	}
 	__device__ __forceinline__ long columns(int vec) const { return (long) (last - first) * vec + (end - tail); }
 };
 
@@ -241,6 +244,56 @@ __device__ __forceinline__ RowPart score_stream(const T * row, const RowSlice & 
 		if (++slot == SCORE_GROUP_SLOTS) { slot = 0; again = true; }
 	}
 	return p;
+}
+
+__device__ __forceinline__ void score_store(void * row, uint64_t uniform_chunk, uint32_t lane_chunk, const R16 & r) {
+	const score_vec v = {r.w[0], r.w[1], r.w[2], r.w[3]};
+	char * p = static_cast<char *>(row) + uniform_chunk * 16u;
+	__builtin_nontemporal_store(v, reinterpret_cast<score_vec *>(p + lane_chunk * 16u));
+}
+
+/* N chunks of out = f(row) */
+template <typename T, int N, typename F>
+__device__ __forceinline__ void score_map_chunks(const T * row, T * out, int c, const F & f) {
+	constexpr int V = VecOf<T>::N;
+	R16 x[N];
+#pragma unroll
+	for (int u = 0; u < N; u++) x[u] = score_load(row, (uint64_t) (c + u * (int) blockDim.x), threadIdx.x);
+#pragma unroll
+	for (int u = 0; u < N; u++) {
+		__builtin_amdgcn_sched_barrier(0);
+		float v[V];
+		unpack16<T>(x[u], v);
+#pragma unroll
+		for (int i = 0; i < V; i++) v[i] = f(v[i]);
+		score_store(out, (uint64_t) (c + u * (int) blockDim.x), threadIdx.x, pack16<T>(v));
+	}
+}
+/* out = f(row) over a slice; out may be row */
+template <typename T, typename F>
+__device__ __forceinline__ void score_map(const T * row, T * out, const RowSlice & sl, const F & f) {
+	const int nt = (int) blockDim.x, tid = (int) threadIdx.x;
+	int c = sl.first;
+	for (; c + SCORE_BATCH * nt <= sl.last; c += SCORE_BATCH * nt) score_map_chunks<T, SCORE_BATCH>(row, out, c, f);
+	if (c + 4 * nt <= sl.last) { score_map_chunks<T, 4>(row, out, c, f); c += 4 * nt; }
+	if (c + 2 * nt <= sl.last) { score_map_chunks<T, 2>(row, out, c, f); c += 2 * nt; }
+	if (c + nt <= sl.last) { score_map_chunks<T, 1>(row, out, c, f); c += nt; }
+	if (c + tid < sl.last) score_map_chunks<T, 1>(row, out, c, f);
+	if (sl.tail + tid < sl.end) out[sl.tail + tid] = from_f<T>(f(to_f(row[sl.tail + tid])));
+}
+/* out = 0 over a slice */
+template <typename T>
+__device__ __forceinline__ void score_clear(T * out, const RowSlice & sl) {
+	R16 zero;
+	zero.w[0] = zero.w[1] = zero.w[2] = zero.w[3] = 0u;
+	for (int c = sl.first + (int) threadIdx.x; c < sl.last; c += (int) blockDim.x) score_store(out, (uint64_t) c, 0u, zero);
+	if (sl.tail + (int) threadIdx.x < sl.end) out[sl.tail + threadIdx.x] = from_f<T>(0.0f);
+}
+/* every store that this workgroup has made so far is done before any that it
+ * makes after this */
+__device__ __forceinline__ void score_stores_done() {
+	__builtin_amdgcn_s_waitcnt(0x0F70);   /* vmcnt(0) */
+	__syncthreads();
 }
 
 template <typename T>

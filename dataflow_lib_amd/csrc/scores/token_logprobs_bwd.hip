@@ -13,54 +13,36 @@ struct GradTokens {
 	uint32_t id[SCORE_TOKENS_MAX];
 	float g[SCORE_TOKENS_MAX], x[SCORE_TOKENS_MAX];
 };
+#define SCORE_NO_TOKEN 0xffffffffu
 
-/* s p (G + h (log p + H)) of a column */
+/* -s p (G + h (log p + H)) of a column */
+template <bool ENTROPY>
 struct GradTerm {
 	float s, lse, down, h, H;
 	__device__ __forceinline__ float operator()(float x) const {
 		const float lp = fmaf(s, x, -lse);
 		const float p = __builtin_amdgcn_exp2f(lp * SCORE_LOG2E);
-		/* h = 0 drops the entropy's term also where log p is -inf */
-		const float f = h != 0.0f ? fmaf(h, fmaxf(lp, -1e30f) + H, down) : down;
-		return -s * p * f;
+		/* the bound keeps -inf * 0 out */
+		return p * (ENTROPY ? -s * fmaf(h, fmaxf(lp, -1e30f) + H, down) : -s * down);
 	}
 };
 
 template <typename T>
-__device__ __forceinline__ void token_logprobs_bwd_run(int n_rows, int n_cols, uint64_t row_stride, uint64_t grad_stride, float s,
-													   int tokens_per_row, const T * logits, const uint32_t * tokens, const float * lse,
-													   const float * entropy, const float * d_logprobs, const float * d_entropy, T * dlogits) {
-	__shared__ float cells[SCORE_MAX_WAVES];
-	__shared__ GradTokens tok;
-	for (long r = blockIdx.x; r < n_rows; r += gridDim.x) {
-		const T * row = logits + (uint64_t) r * row_stride;
-		T * out = dlogits + (uint64_t) r * grad_stride;
-		__syncthreads();
-		float down = 0.0f, any = 0.0f;
-		for (int m = (int) threadIdx.x; m < tokens_per_row; m += (int) blockDim.x) {
-			const uint32_t t = tokens[r * tokens_per_row + m];
-			const bool is = t < (uint32_t) n_cols;
-			const float g = is ? d_logprobs[r * tokens_per_row + m] : 0.0f;
-			tok.id[m] = is ? t : 0xffffffffu;
-			tok.g[m] = g;
-			tok.x[m] = is ? to_f(row[t]) : 0.0f;
-			down += g;
-			any = g != 0.0f ? 1.0f : any;
-		}
-		down = score_group_sum(down, cells);
-		any = score_group_max(any, cells);
-		GradTerm term = {s, lse[r], down, d_entropy ? d_entropy[r] : 0.0f, d_entropy ? entropy[r] : 0.0f};
-		if ((any == 0.0f && term.h == 0.0f) || term.lse == -__builtin_inff()) {
-			for (long j = threadIdx.x; j < n_cols; j += blockDim.x) out[j] = from_f<T>(0.0f);
-			continue;
-		}
-		for (long j = threadIdx.x; j < n_cols; j += blockDim.x) out[j] = from_f<T>(term(to_f(row[j])));
-		__threadfence_block();
-		__builtin_amdgcn_s_waitcnt(0);
-		__syncthreads();
+struct GradRow {
+	const T * row;
+	T * out;
+	int tokens_per_row;
+	RowSlice sl;
+	GradTokens & tok;
+
+	template <typename F>
+	__device__ __forceinline__ void run(const F & term, float s) const {
+		score_map(row, out, sl, term);
+		if (tokens_per_row == 0) return;
+		score_stores_done();
 		for (int m = (int) threadIdx.x; m < tokens_per_row; m += (int) blockDim.x) {
 			const uint32_t t = tok.id[m];
-			if (t == 0xffffffffu) continue;
+			if (t == SCORE_NO_TOKEN || !sl.holds(t, VecOf<T>::N)) continue;
 			float g = 0.0f;
 			bool first = true;
 			for (int o = 0; o < tokens_per_row; o++)
@@ -71,10 +53,53 @@ __device__ __forceinline__ void token_logprobs_bwd_run(int n_rows, int n_cols, u
 			if (first) out[t] = from_f<T>(fmaf(s, g, term(tok.x[m])));
 		}
 	}
+};
+
+template <typename T>
+__device__ __forceinline__ void token_logprobs_bwd_run(int n_rows, int n_cols, uint64_t row_stride, uint64_t grad_stride, float s,
+													   int tokens_per_row, const T * logits, const uint32_t * tokens, const float * lse,
+													   const float * entropy, const float * d_logprobs, const float * d_entropy, T * dlogits) {
+	constexpr int V = VecOf<T>::N;
+	__shared__ float cells[SCORE_MAX_WAVES];
+	__shared__ GradTokens tok;
+	const Score_Plan plan = score_map_plan(n_rows, n_cols, (int) sizeof(T));
+	for (long w = blockIdx.x; w < (long) n_rows * plan.slices; w += gridDim.x) {
+		const long r = plan.slices == 1 ? w : w / plan.slices;
+		const int slice = plan.slices == 1 ? 0 : (int) (w - r * plan.slices);
+		const RowSlice sl(n_cols, V, slice, plan.slices, plan.slice_chunks);
+		const T * row = logits + (uint64_t) r * row_stride;
+		T * out = dlogits + (uint64_t) r * grad_stride;
+		__syncthreads();
+		float down = 0.0f, any = 0.0f;
+		for (int m = (int) threadIdx.x; m < tokens_per_row; m += (int) blockDim.x) {
+			const uint32_t t = tokens[r * tokens_per_row + m];
+			const bool is = t < (uint32_t) n_cols;
+			const float g = is ? d_logprobs[r * tokens_per_row + m] : 0.0f;
+			tok.id[m] = is ? t : SCORE_NO_TOKEN;
+			tok.g[m] = g;
+			tok.x[m] = is && sl.holds(t, V) ? to_f(row[t]) : 0.0f;
+			down += g;
+			any = g != 0.0f ? 1.0f : any;
+		}
+		if (tokens_per_row == 1) {
+			__syncthreads();
+			down = tok.g[0];
+			any = down != 0.0f ? 1.0f : 0.0f;
+		}
+		else {
+			down = score_group_sum(down, cells);
+			any = score_group_max(any, cells);
+		}
+		const float row_lse = lse[r], h = d_entropy ? d_entropy[r] : 0.0f, H = d_entropy ? entropy[r] : 0.0f;
+		const GradRow<T> g = {row, out, tokens_per_row, sl, tok};
+		if ((any == 0.0f && h == 0.0f) || row_lse == -__builtin_inff()) score_clear(out, sl);
+		else if (h != 0.0f) g.run(GradTerm<true>{s, row_lse, down, h, H}, s);
+		else g.run(GradTerm<false>{s, row_lse, down, h, H}, s);
+	}
 }
 
 #define TOKEN_LOGPROBS_BWD_KERNEL(SUF, T)                                                                                      \
-	extern "C" __global__ void __launch_bounds__(SCORE_THREADS) token_logprobs_bwd_##SUF##_kernel(int n_rows, int n_cols,      \
+	extern "C" __global__ void __launch_bounds__(64 * SCORE_MAP_WAVES) token_logprobs_bwd_##SUF##_kernel(int n_rows, int n_cols,      \
 			uint64_t row_stride, uint64_t grad_stride, float scale, int tokens_per_row, T * logits, uint32_t * tokens,         \
 			float * lse, float * entropy, float * d_logprobs, float * d_entropy, T * dlogits) {                                \
 		token_logprobs_bwd_run<T>(n_rows, n_cols, row_stride, grad_stride, scale, tokens_per_row, logits, tokens, lse,         \
