@@ -81,9 +81,21 @@ static void plan_config(Hip_Launch_Config * c, Score_Plan plan, int n_rows, unsi
 	set_1d(c, (unsigned) MY_MIN((long) n_rows * plan.slices, (long) SCORE_MAX_GROUPS), (unsigned) (64 * plan.waves), lds);
 }
 
-/* one workgroup per row */
-static void rows_config(Hip_Launch_Config * c, int n_rows) {
-	set_1d(c, (unsigned) MY_MIN(n_rows, SCORE_MAX_GROUPS), SCORE_THREADS, 0);
+/* workgroups of one of this function's kernels that are resident on the whole
+ * device at once; the occupancy query is remembered per kernel for the last
+ * (block, LDS) pair asked */
+static long resident_groups(Dataflow_Handle * h, Hip_Function * f, unsigned variant, int block, unsigned lds) {
+	uint64_t * slot = &f->function_config.occupancy_memo[variant];
+	const uint64_t key = ((uint64_t) (unsigned) block << 40) | ((uint64_t) lds << 16);
+	const uint64_t memo = __atomic_load_n(slot, __ATOMIC_RELAXED);
+	int per_cu = 0;
+	if (memo != 0 && (memo & ~0xffffull) == key) per_cu = (int) (memo & 0xffffull);
+	else {
+		const hipFunction_t fn = f->variant_handles[variant - 1];
+		if (!fn || hipModuleOccupancyMaxActiveBlocksPerMultiprocessor(&per_cu, fn, block, lds) != hipSuccess || per_cu < 1) per_cu = 1;
+		if (per_cu <= 0xffff) __atomic_store_n(slot, key | (uint64_t) per_cu, __ATOMIC_RELAXED);
+	}
+	return (long) per_cu * (long) ((const Hip_Device_Info *) h->device_info)->cu_count;
 }
 
 int token_logprobs_set_launch_config(Hip_Launch_Config * hip_launch_config, Dataflow_Handle * dataflow_handle, Hip_Function * hip_function, Op * op) {
@@ -154,7 +166,6 @@ int token_logprobs_bwd_set_launch_config(Hip_Launch_Config * hip_launch_config, 
 }
 
 int distillation_loss_set_launch_config(Hip_Launch_Config * hip_launch_config, Dataflow_Handle * dataflow_handle, Hip_Function * hip_function, Op * op) {
-	(void) dataflow_handle;
 	const char * what = "distillation loss";
 	const int n_rows = ARG(op, 0, int), n_cols = ARG(op, 1, int), top_k = ARG(op, 5, int);
 	const size_t elem = logits_elem(hip_function);
@@ -175,7 +186,18 @@ int distillation_loss_set_launch_config(Hip_Launch_Config * hip_launch_config, D
 	if (ARG(op, 11, void *) && score_pointer(what, "the mean loss pointer", ARG(op, 11, void *), 4)) return -1;
 	if (ARG(op, 12, void *) && score_check_grad(what, n_rows, n_cols, ARG(op, 2, uint64_t), ARG(op, 3, uint64_t), ARG(op, 6, void *), ARG(op, 12, void *), elem)) return -1;
 	if (score_check_workspace(what, score_distill_workspace(n_rows, n_cols, (int) elem, top_k), ARG(op, 13, uint64_t), ARG(op, 14, void *))) return -1;
-	rows_config(hip_launch_config, n_rows);
+	const int held = ARG(op, 12, void *) ? score_held(n_rows, n_cols, (int) elem, top_k) : 0;
+	if (held) {
+		const int waves = score_held_waves(held, n_cols, (int) elem, top_k);
+		const unsigned lds = (unsigned) (2 * 8 * top_k);
+		const unsigned variant = held == SCORE_HELD ? HIP_VARIANT_ROWS : HIP_VARIANT_WIDE_ROWS;
+		set_1d(hip_launch_config, (unsigned) MY_MIN((long) n_rows, resident_groups(dataflow_handle, hip_function, variant, 64 * waves, lds)), (unsigned) (64 * waves), lds);
+		hip_launch_config->variant = variant;
+		return 0;
+	}
+	const Score_Plan plan = score_stream_plan(n_rows, n_cols, (int) elem);
+	plan_config(hip_launch_config, plan, n_rows, 0);
+	if (plan.slices > 1 || ARG(op, 12, void *)) hip_launch_config->then_variant = HIP_VARIANT_SPLIT_OUT;
 	return 0;
 }
 

@@ -88,9 +88,32 @@ GEOM_FN unsigned long score_logprobs_workspace(int n_rows, int n_cols, int elem_
 	return (unsigned long) n_rows * (unsigned long) p.slices * (sizeof(Score_Part) + 8ul * (unsigned long) top_k);
 }
 
-GEOM_FN unsigned long score_distill_workspace(int n_rows, int n_cols, int elem_bytes, int top_k) {
-	(void) n_rows; (void) n_cols; (void) elem_bytes; (void) top_k;
+/* distillation_loss with a gradient: rows that a workgroup holds in its
+ * registers, SCORE_HELD or SCORE_HELD_WIDE chunks per thread, with a thread per
+ * teacher entry. 0: not held. */
+#define SCORE_HELD 4
+#define SCORE_HELD_WIDE 16
+#define SCORE_HELD_FEW 128
+GEOM_FN int score_held_waves(int held, int n_cols, int elem_bytes, int top_k) {
+	const long chunks = (long) n_cols * elem_bytes / 16;
+	long waves = (chunks + 64 * held - 1) / (64 * held);
+	const long entries = (top_k + 63) / 64;
+	if (waves < entries) waves = entries;
+	if (waves < 1) waves = 1;
+	return waves <= 16 ? (int) waves : 0;
+}
+GEOM_FN int score_held(int n_rows, int n_cols, int elem_bytes, int top_k) {
+	if (score_held_waves(SCORE_HELD, n_cols, elem_bytes, top_k) > 0) return SCORE_HELD;
+	if (n_rows >= SCORE_HELD_FEW && score_held_waves(SCORE_HELD_WIDE, n_cols, elem_bytes, top_k) > 0) return SCORE_HELD_WIDE;
 	return 0;
+}
+
+/* a call may want the loss alone, whatever its sizes */
+GEOM_FN unsigned long score_distill_workspace(int n_rows, int n_cols, int elem_bytes, int top_k) {
+	if (n_rows <= 0 || n_cols <= 0 || elem_bytes <= 0 || top_k < 0) return 0;
+	const Score_Plan p = score_stream_plan(n_rows, n_cols, elem_bytes);
+	if (p.slices == 1 && score_held(n_rows, n_cols, elem_bytes, top_k)) return 0;
+	return (unsigned long) n_rows * ((unsigned long) p.slices * sizeof(Score_Part) + 4ul * (unsigned long) top_k);
 }
 
 /* token_logprobs: LDS of a workgroup with alternatives to find. Group maxima
