@@ -51,17 +51,25 @@ struct DistillCells {
 	float m[SCORE_MAX_WAVES], z[SCORE_MAX_WAVES], vm[SCORE_MAX_WAVES], vz[SCORE_MAX_WAVES], loss[SCORE_MAX_WAVES];
 };
 
+/* a row's parts, one per wave, joined by the lanes of each wave alike: lane i
+ * takes cell i of 16, and all rows of 16 lanes end with the total */
 __device__ __forceinline__ RowPart join_cells(const float * m, const float * z, int waves, float s_log2e) {
-	RowPart sum;
-	for (int w = 0; w < waves; w++) sum.m = fmaxf(sum.m, m[w]);
-	for (int w = 0; w < waves; w++) {
-		RowPart q;
-		q.m = m[w];
-		q.z = z[w];
-		q.shift(sum.m, s_log2e);
-		sum.z += q.z;
-	}
-	return sum;
+	const int i = (int) threadIdx.x & 15;
+	RowPart p;
+	p.m = i < waves ? m[i] : -__builtin_inff();
+	p.z = i < waves ? z[i] : 0.0f;
+	float t = fmaxf(p.m, dpp_f32<DPP_QUAD_1032>(p.m));
+	t = fmaxf(t, dpp_f32<DPP_QUAD_2301>(t));
+	t = fmaxf(t, dpp_f32<DPP_ROW_HALF_MIRROR>(t));
+	t = fmaxf(t, dpp_f32<DPP_ROW_MIRROR>(t));
+	p.shift(t, s_log2e);
+	p.z += dpp_f32<DPP_QUAD_1032>(p.z);
+	p.z += dpp_f32<DPP_QUAD_2301>(p.z);
+	p.z += dpp_f32<DPP_ROW_HALF_MIRROR>(p.z);
+	p.z += dpp_f32<DPP_ROW_MIRROR>(p.z);
+	p.m = readlane_f32(p.m, 0);
+	p.z = readlane_f32(p.z, 0);
+	return p;
 }
 
 template <typename T> __device__ __forceinline__ float buf_load_elem(__amdgpu_buffer_rsrc_t r, uint32_t off);
@@ -96,15 +104,16 @@ template <> __device__ __forceinline__ void buf_store_elem<bf16_t>(__amdgpu_buff
  * when a thread has a row's last chunk its stores of the row before are done;
  * behind the next barrier everybody's are, and there the teacher's columns of
  * that row are stored, and its loss. */
-template <typename T, int CH>
+template <typename T, int CH, int NT>
 __device__ __forceinline__ void distill_held(const DistillArgs & a) {
 	constexpr int V = VecOf<T>::N;
 	constexpr uint32_t E = (uint32_t) sizeof(T);
 	constexpr int B = CH < 4 ? CH : 4;   /* chunks that share a shift */
 	__shared__ DistillCells both[2];
 	extern __shared__ uint32_t entries[];   /* ids and values of two rows */
-	const int tid = (int) threadIdx.x, nt = (int) blockDim.x, wave = tid >> 6, waves = nt >> 6, K = a.top_k;
-	const int chunks = a.n_cols / V, whole = chunks / nt, part = chunks - whole * nt;
+	const int tid = (int) threadIdx.x, nt = NT ? NT : (int) blockDim.x, wave = tid >> 6, waves = nt >> 6, K = a.top_k;
+	const int chunks = a.n_cols / V, whole = chunks / nt;
+	const int have = whole + (tid < chunks - whole * nt ? 1 : 0);   /* this thread's chunks */
 	const float s_log2e = a.s * SCORE_LOG2E, temperature = 1.0f / a.s;
 	const uint32_t voff = (uint32_t) tid * 16u;
 	const uint32_t tail_off = chunks * V + tid < a.n_cols ? (uint32_t) (chunks * V + tid) * E : SCORE_NOWHERE;
@@ -146,7 +155,7 @@ __device__ __forceinline__ void distill_held(const DistillArgs & a) {
 		const uint32_t next_id = __builtin_amdgcn_raw_buffer_load_b32(ids_rsrc(next), entry_off, 0, 0);
 		const float next_v = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(values_rsrc(next), entry_off, 0, 0));
 
-		/* statistics; chunks that the row does not have become -inf */
+		/* statistics */
 		RowPart p;
 		const float xtail = tail_off != SCORE_NOWHERE ? xt : -__builtin_inff();
 		p.m = fmaxf(xtail, -__builtin_inff());
@@ -156,13 +165,7 @@ __device__ __forceinline__ void distill_held(const DistillArgs & a) {
 			float m = -__builtin_inff();
 #pragma unroll
 			for (int j = j0; j < j0 + B; j++) {
-				reg_barrier(x[j]);
-				if (j >= whole && (j > whole || tid >= part)) {
-					float none[V];
-#pragma unroll
-					for (int i = 0; i < V; i++) none[i] = -__builtin_inff();
-					x[j] = pack16<T>(none);
-				}
+				if (j >= have) continue;
 				float f[V];
 				unpack16<T>(x[j], f);
 #pragma unroll
@@ -173,6 +176,7 @@ __device__ __forceinline__ void distill_held(const DistillArgs & a) {
 			float z[2] = {0.0f, 0.0f};
 #pragma unroll
 			for (int j = j0; j < j0 + B; j++) {
+				if (j >= have) continue;
 				__builtin_amdgcn_sched_barrier(0);
 				reg_barrier(x[j]);
 				float f[V];
@@ -228,6 +232,7 @@ __device__ __forceinline__ void distill_held(const DistillArgs & a) {
 				if (!(q == 0.0f)) l = q * ((d - logf(te.z)) - (st.none() ? -__builtin_inff() : st.log_p(xk, a.s)));
 				bool first = true;
 				float sum = 0.0f;
+#pragma unroll 1
 				for (int o = 0; o < K; o++) {
 					if (ids[o] != id) continue;
 					if (o < tid) first = false;
@@ -443,14 +448,18 @@ __device__ __forceinline__ void distillation_loss_mean(int n_rows, const float *
 					 loss, dlogits, static_cast<Score_Part *>(workspace), nullptr};                                              \
 	a.picked = reinterpret_cast<float *>(a.parts + (uint64_t) n_rows * score_stream_plan(n_rows, n_cols, (int) sizeof(*logits)).slices);
 #define DISTILLATION_LOSS_KERNEL(SUF, T)                                                                                         \
-	extern "C" __global__ void __launch_bounds__(1024) distillation_loss_##SUF##_kernel_wide_rows(DISTILLATION_ARGS(T)) {        \
-		DISTILLATION_PACK                                                                                                        \
-		distill_held<T, SCORE_HELD_WIDE>(a);                                                                                     \
-	}                                                                                                                            \
-	extern "C" __global__ void __launch_bounds__(1024) distillation_loss_##SUF##_kernel_rows(DISTILLATION_ARGS(T)) {             \
-		DISTILLATION_PACK                                                                                                        \
-		distill_held<T, SCORE_HELD>(a);                                                                                          \
-	}                                                                                                                            \
+	extern "C" __global__ void __launch_bounds__(1024) distillation_loss_##SUF##_kernel_long_rows(DISTILLATION_ARGS(T)) { \
+		DISTILLATION_PACK \
+		distill_held<T, SCORE_HELD_MORE, 1024>(a); \
+	} \
+	extern "C" __global__ void __launch_bounds__(512, 2) distillation_loss_##SUF##_kernel_wide_rows(DISTILLATION_ARGS(T)) { \
+		DISTILLATION_PACK \
+		distill_held<T, SCORE_HELD_MORE, 512>(a); \
+	} \
+	extern "C" __global__ void __launch_bounds__(1024) distillation_loss_##SUF##_kernel_rows(DISTILLATION_ARGS(T)) { \
+		DISTILLATION_PACK \
+		distill_held<T, SCORE_HELD, 0>(a); \
+	} \
 	extern "C" __global__ void __launch_bounds__(64 * SCORE_STREAM_WAVES) distillation_loss_##SUF##_kernel(DISTILLATION_ARGS(T)) { \
 		DISTILLATION_PACK                                                                                                        \
 		distill_parts<T>(a);                                                                                                     \

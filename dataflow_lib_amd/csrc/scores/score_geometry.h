@@ -89,23 +89,28 @@ GEOM_FN unsigned long score_logprobs_workspace(int n_rows, int n_cols, int elem_
 }
 
 /* distillation_loss with a gradient: rows that a workgroup holds in its
- * registers, SCORE_HELD or SCORE_HELD_WIDE chunks per thread, with a thread per
- * teacher entry. 0: not held. */
+ * registers, with a thread per teacher entry. SCORE_HELD_ROWS: SCORE_HELD
+ * chunks per thread and as many waves as that takes; SCORE_HELD_WIDE_ROWS and
+ * SCORE_HELD_LONG_ROWS: SCORE_HELD_MORE chunks per thread, 8 and 16 waves. */
 #define SCORE_HELD 4
-#define SCORE_HELD_WIDE 16
+#define SCORE_HELD_MORE 16
 #define SCORE_HELD_FEW 128
-GEOM_FN int score_held_waves(int held, int n_cols, int elem_bytes, int top_k) {
-	const long chunks = (long) n_cols * elem_bytes / 16;
-	long waves = (chunks + 64 * held - 1) / (64 * held);
-	const long entries = (top_k + 63) / 64;
-	if (waves < entries) waves = entries;
-	if (waves < 1) waves = 1;
-	return waves <= 16 ? (int) waves : 0;
-}
+#define SCORE_HELD_NONE 0
+#define SCORE_HELD_ROWS 1
+#define SCORE_HELD_WIDE_ROWS 2
+#define SCORE_HELD_LONG_ROWS 3
 GEOM_FN int score_held(int n_rows, int n_cols, int elem_bytes, int top_k) {
-	if (score_held_waves(SCORE_HELD, n_cols, elem_bytes, top_k) > 0) return SCORE_HELD;
-	if (n_rows >= SCORE_HELD_FEW && score_held_waves(SCORE_HELD_WIDE, n_cols, elem_bytes, top_k) > 0) return SCORE_HELD_WIDE;
-	return 0;
+	const long chunks = (long) n_cols * elem_bytes / 16;
+	if (chunks <= 16 * 64 * SCORE_HELD) return SCORE_HELD_ROWS;
+	if (n_rows < SCORE_HELD_FEW) return SCORE_HELD_NONE;
+	if (chunks <= 8 * 64 * SCORE_HELD_MORE && top_k <= 8 * 64) return SCORE_HELD_WIDE_ROWS;
+	return chunks <= 16 * 64 * SCORE_HELD_MORE ? SCORE_HELD_LONG_ROWS : SCORE_HELD_NONE;
+}
+GEOM_FN int score_held_waves(int held, int n_cols, int elem_bytes, int top_k) {
+	if (held != SCORE_HELD_ROWS) return held == SCORE_HELD_WIDE_ROWS ? 8 : 16;
+	const int chunks = (int) ((long) n_cols * elem_bytes / 16);
+	const int waves = (chunks + 64 * SCORE_HELD - 1) / (64 * SCORE_HELD), entries = (top_k + 63) / 64;
+	return waves > entries ? waves : entries > 0 ? entries : 1;
 }
 
 /* a call may want the loss alone, whatever its sizes */

@@ -297,7 +297,7 @@ def test_workspaces_are_checked(op, dt):
         assert config(op, dt, workspaceBytes=need, workspace=0x40000000 if need else None, **call)[0] == 0
         if need:
             asked += 1
-            assert need <= 64 << 20
+            assert need <= rows * (32 * 16 + (4 * k if op == "distillation_loss" else 32 * 8 * k))
             for space in ((need - 1, 0x40000000), (need, None), (need, 0x40000010), (0, None)):
                 assert config(op, dt, workspaceBytes=space[0], workspace=space[1], **call)[0] == -1
     assert size(dt, 0, 100, 5) == 0 and size(dt, 4, 0, 0) == 0 and size(dt, -1, -1, -1) == 0
