@@ -135,7 +135,7 @@ int token_logprobs_set_finish_launch_config(Hip_Launch_Config * hip_launch_confi
 	(void) dataflow_handle;
 	const int n_rows = ARG(op, 0, int), top_k = ARG(op, 5, int);
 	const Score_Plan plan = score_stream_plan(n_rows, ARG(op, 1, int), (int) logits_elem(hip_function));
-	set_1d(hip_launch_config, plan.slices > 1 ? (unsigned) n_rows : 0u, SCORE_THREADS, (unsigned) (8 * plan.slices * top_k));
+	set_1d(hip_launch_config, plan.slices > 1 ? (unsigned) n_rows : 0u, SCORE_JOIN_THREADS, (unsigned) (8 * plan.slices * top_k));
 	return 0;
 }
 

@@ -35,7 +35,8 @@
 #define SCORE_MAP_BATCH 2
 /* few rows: slices until the chip has this many waves */
 #define SCORE_FILL_WAVES 2048
-#define SCORE_MAX_SLICES 32
+#define SCORE_MAX_SLICES 32   /* fewer than a wave's lanes, one of which joins each */
+#define SCORE_JOIN_THREADS 512
 
 /* how a call's rows are cut */
 typedef struct {
@@ -121,12 +122,12 @@ GEOM_FN unsigned long score_distill_workspace(int n_rows, int n_cols, int elem_b
 	return (unsigned long) n_rows * ((unsigned long) p.slices * sizeof(Score_Part) + 4ul * (unsigned long) top_k);
 }
 
-/* token_logprobs: LDS of a workgroup with alternatives to find. Group maxima
- * (SCORE_GROUP_SLOTS per thread) and candidates. */
+/* token_logprobs: LDS of a workgroup with alternatives to find. Candidates,
+ * group maxima (SCORE_GROUP_SLOTS per thread) and which of them reach a bound. */
 #define SCORE_GROUP_SLOTS 4
 #define SCORE_CANDIDATES 1024
 GEOM_FN unsigned score_top_lds(int waves) {
-	return (unsigned) (waves * 64 * SCORE_GROUP_SLOTS * 4 + SCORE_CANDIDATES * 8);
+	return (unsigned) (waves * 64 * SCORE_GROUP_SLOTS * 6 + SCORE_CANDIDATES * 8);
 }
 
 #endif

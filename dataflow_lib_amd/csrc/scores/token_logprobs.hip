@@ -19,7 +19,7 @@ struct TopState {
 	float cells[3 * SCORE_MAX_WAVES];
 	uint32_t counts[2 * SCORE_MAX_WAVES];
 	uint32_t hist[256];
-	uint32_t prefix, need, count;
+	uint32_t prefix, need, count, n_groups;
 };
 
 /* a count over a workgroup of a wave's count; calls alternate between two
@@ -99,7 +99,7 @@ __device__ __forceinline__ void score_select(const T * row, int first, int end, 
  * them (all of them where there are fewer than k). `groups`: the maxima that
  * the thread's batches left, SCORE_GROUP_SLOTS rows of blockDim.x. Returns n. */
 template <typename T>
-__device__ __forceinline__ int score_candidates(const T * row, const RowSlice & sl, int k, float row_max, const float * groups, uint64_t * list, TopState & t) {
+__device__ __forceinline__ int score_candidates(const T * row, const RowSlice & sl, int k, float row_max, const float * groups, uint16_t * reached, uint64_t * list, TopState & t) {
 	constexpr int V = VecOf<T>::N;
 	const int tid = (int) threadIdx.x, nt = (int) blockDim.x;
 	const int batches = (sl.last - sl.first + SCORE_BATCH * nt - 1) / (SCORE_BATCH * nt);
@@ -126,38 +126,51 @@ __device__ __forceinline__ int score_candidates(const T * row, const RowSlice & 
 		mine = fmaxf(mine, g[i]);
 	}
 	int turn = 0;
-	__syncthreads();
-	if (tid == 0) t.count = 0u;
 	/* as many threads as have a column above -inf reach the least of their maxima */
 	const bool has = mine > -__builtin_inff();
 	float lo = -score_group_max(has ? -mine : -__builtin_inff(), t.cells);
-	float hi = row_max;
-	if (score_group_count((uint32_t) __popcll(__ballot(has)), t, turn) >= (uint32_t) k) {
-		/* lo is reached by k groups or more, hi not known to be */
-		for (int step = 0; step < 24; step++) {
-			const float mid = 0.5f * lo + 0.5f * hi;
-			if (!(mid > lo)) break;
+	if (tid == 0) t.count = t.n_groups = 0u;
+	uint32_t reach = score_group_count((uint32_t) __popcll(__ballot(has)), t, turn);
+	if (reach >= (uint32_t) k) {
+		/* lo is reached by k groups or more, hi not known to be. Far from a row's
+		 * bulk the logarithm of how many reach a bound falls about evenly, so every
+		 * other bound is interpolated there; the others halve the interval. */
+		float hi = row_max, at_hi = 0.0f;
+		const float aim = __builtin_amdgcn_logf(1.25f * (float) k + 2.0f);
+		for (int step = 0; step < 24 && reach > (uint32_t) (k + (k >> 1) + 8); step++) {
+			const float at_lo = __builtin_amdgcn_logf((float) reach);
+			float part = 0.5f;
+			if (!(step & 1)) part = fminf(fmaxf((at_lo - aim) / (at_lo - at_hi), 0.02f), 0.98f);
+			const float mid = lo + part * (hi - lo);
+			if (!(mid > lo && mid <= hi)) break;
 			uint32_t n = 0;
 #pragma unroll
 			for (int i = 0; i < SCORE_GROUP_SLOTS; i++) n += (uint32_t) __popcll(__ballot(g[i] >= mid));
 			n = score_group_count(n, t, turn);
-			if (n < (uint32_t) k) hi = mid;
+			if (n < (uint32_t) k) {
+				hi = mid;
+				at_hi = n == 0u ? 0.0f : __builtin_amdgcn_logf((float) n);
+			}
 			else {
 				lo = mid;
-				if (n <= (uint32_t) (k + (k >> 1) + 8)) break;
+				reach = n;
 			}
 		}
 	}
 	else lo = -3.402823466e38f;   /* few columns are above -inf: all of them */
+	/* the groups that reach it, and then a thread for each of their chunks */
+#pragma unroll
+	for (int i = 0; i < SCORE_GROUP_SLOTS; i++)
+		if (g[i] >= lo) reached[atomicAdd(&t.n_groups, 1u)] = (uint16_t) (i * nt + tid);
+	__syncthreads();
+	const int items = (int) t.n_groups * SCORE_BATCH;
 #pragma unroll 1
-	for (int i = 0; i < SCORE_GROUP_SLOTS; i++) {
-		if (!((i < batches || i == 0 ? groups[i * nt + tid] : -__builtin_inff()) >= lo)) continue;
+	for (int item = tid; item < items; item += nt) {
+		const int group = reached[item / SCORE_BATCH], slot = group / nt, owner = group - slot * nt;
 #pragma unroll 1
-		for (int b = i; b < batches; b += SCORE_GROUP_SLOTS)
-#pragma unroll 1
-			for (int u = 0; u < SCORE_BATCH; u++) {
-				const int c = sl.first + (b * SCORE_BATCH + u) * nt + tid;
-				if (c >= sl.last) break;
+		for (int b = slot; b < batches || b == 0; b += SCORE_GROUP_SLOTS) {
+			const int c = sl.first + (b * SCORE_BATCH + item % SCORE_BATCH) * nt + owner;
+			if (c < sl.last) {
 				const R16 x = score_load(row, (uint64_t) c, 0u);
 				float f[V];
 				unpack16<T>(x, f);
@@ -168,9 +181,13 @@ __device__ __forceinline__ int score_candidates(const T * row, const RowSlice & 
 						if (at < SCORE_CANDIDATES) list[at] = score_alternative(score_key(f[v]), (uint32_t) (c * V + v));
 					}
 			}
-		if (i == 0 && tail && to_f(row[sl.tail + tid]) >= lo) {
+		}
+	}
+	if (tail) {
+		const float x = to_f(row[sl.tail + tid]);
+		if (x >= lo) {
 			const uint32_t at = atomicAdd(&t.count, 1u);
-			if (at < SCORE_CANDIDATES) list[at] = score_alternative(score_key(to_f(row[sl.tail + tid])), (uint32_t) (sl.tail + tid));
+			if (at < SCORE_CANDIDATES) list[at] = score_alternative(score_key(x), (uint32_t) (sl.tail + tid));
 		}
 	}
 	__syncthreads();
@@ -191,11 +208,20 @@ __device__ __forceinline__ int score_candidates(const T * row, const RowSlice & 
 	return n;
 }
 
-/* how many of a list's n numbers exceed one of them */
-__device__ __forceinline__ int score_rank(const uint64_t * list, int n, uint64_t a) {
-	int r = 0;
-	for (int o = 0; o < n; o++) r += list[o] > a ? 1 : 0;
-	return r;
+/* The place of each of a list's n numbers among them, by counting the larger
+ * ones: four threads a number, each over a quarter of the list. put(place,
+ * number) is called by one of them. */
+template <typename Put>
+__device__ __forceinline__ void score_rank(const uint64_t * list, int n, const Put & put) {
+	for (int i = (int) threadIdx.x >> 2; i < n; i += (int) (blockDim.x >> 2)) {
+		const uint64_t alt = list[i];
+		int r = 0;
+#pragma unroll 4
+		for (int o = (int) threadIdx.x & 3; o < n; o += 4) r += list[o] > alt ? 1 : 0;
+		r += __builtin_amdgcn_update_dpp(0, r, DPP_QUAD_1032, 0xf, 0xf, false);
+		r += __builtin_amdgcn_update_dpp(0, r, DPP_QUAD_2301, 0xf, 0xf, false);
+		if ((threadIdx.x & 3) == 0) put(r, alt);
+	}
 }
 
 struct LogprobsArgs {
@@ -231,6 +257,7 @@ __device__ __forceinline__ void token_logprobs_run(const LogprobsArgs & a) {
 	__shared__ TopState t;
 	extern __shared__ uint64_t list[];
 	float * groups = reinterpret_cast<float *>(list + SCORE_CANDIDATES);
+	uint16_t * reached = reinterpret_cast<uint16_t *>(groups + SCORE_GROUP_SLOTS * blockDim.x);
 	const Score_Plan plan = score_stream_plan(a.n_rows, a.n_cols, (int) sizeof(T));
 	const int tid = (int) threadIdx.x, nt = (int) blockDim.x;
 	const float s_log2e = a.s * SCORE_LOG2E;
@@ -246,17 +273,15 @@ __device__ __forceinline__ void token_logprobs_run(const LogprobsArgs & a) {
 		else if (tid == 0) a.parts[w] = Score_Part{p.m, p.z, p.e, 0.0f};
 		if (a.top_k > 0) {
 			const int k = a.top_k;
-			const int n = score_candidates(row, sl, k, p.m, groups, list, t);
-			for (int i = tid; i < n; i += nt) {
-				const uint64_t alt = list[i];
-				const int rank = score_rank(list, n, alt);
-				if (rank >= k) continue;
+			const int n = score_candidates(row, sl, k, p.m, groups, reached, list, t);
+			score_rank(list, n, [&](int rank, uint64_t alt) {
+				if (rank >= k) return;
 				if (plan.slices == 1) {
 					a.top_ids[r * k + rank] = score_alternative_id(alt);
 					a.top_logprobs[r * k + rank] = st.log_p(score_alternative_value(alt), a.s);
 				}
 				else a.lists[w * k + rank] = alt;
-			}
+			});
 			if (plan.slices > 1)
 				for (int i = n + tid; i < k; i += nt) a.lists[w * k + i] = 0u;
 		}
@@ -264,56 +289,54 @@ __device__ __forceinline__ void token_logprobs_run(const LogprobsArgs & a) {
 	}
 }
 
-/* A row's slices, joined: one workgroup per row. An alternative's rank is the
- * sum over the slices' sorted lists of how many of each exceed it. */
+/* A row's slices, joined: one workgroup per row. k of the slices' alternatives
+ * or more reach any slice's k-th, and the least of their p-th ones with
+ * p = k / slices, rounded up: those that reach both are ranked by counting. */
 template <typename T>
 __device__ __forceinline__ void token_logprobs_join(const LogprobsArgs & a) {
 	extern __shared__ uint64_t list[];
+	__shared__ uint32_t count;
+	__shared__ unsigned long long all_reach, one_reaches;
 	const Score_Plan plan = score_stream_plan(a.n_rows, a.n_cols, (int) sizeof(T));
-	const int tid = (int) threadIdx.x, nt = (int) blockDim.x, k = a.top_k, slices = plan.slices;
+	const int tid = (int) threadIdx.x, nt = (int) blockDim.x, lane = tid & 63, k = a.top_k, slices = plan.slices;
 	const float s_log2e = a.s * SCORE_LOG2E;
 	for (long r = blockIdx.x; r < a.n_rows; r += gridDim.x) {
 		const T * row = static_cast<const T *>(a.logits) + (uint64_t) r * a.row_stride;
-		const Score_Part * parts = a.parts + r * slices;
-		float m = -__builtin_inff();
-		for (int i = 0; i < slices; i++) m = fmaxf(m, parts[i].max);
-		RowPart p;
-		p.m = m;
-		for (int i = 0; i < slices; i++) {
-			RowPart q;
-			q.m = parts[i].max;
-			q.z = parts[i].z;
-			q.e = parts[i].e;
-			q.shift(m, s_log2e);
-			p.z += q.z;
-			p.e += q.e;
+		const uint64_t * lists = a.lists + r * slices * k;
+		RowPart p;   /* a lane of each wave for a slice (SCORE_MAX_SLICES are fewer than lanes) */
+		if (lane < slices) {
+			const Score_Part q = a.parts[r * slices + lane];
+			p.m = q.max;
+			p.z = q.z;
+			p.e = q.e;
 		}
+		if (k > 0) {
+			if (tid == 0) { count = 0u; all_reach = ~0ull; one_reaches = 0ull; }
+			__syncthreads();
+			if (tid < slices) {
+				atomicMax(&one_reaches, (unsigned long long) lists[tid * k + k - 1]);
+				atomicMin(&all_reach, (unsigned long long) lists[tid * k + (k + slices - 1) / slices - 1]);
+			}
+		}
+		p.shift(wave_max(p.m), s_log2e);
+		p.z = wave_sum(p.z);
+		p.e = wave_sum(p.e);
 		const RowStats st(p.m, p.z, p.e);
 		token_logprobs_row<T>(a, r, row, st);
+		if (k == 0) continue;
 		__syncthreads();
-		for (int i = tid; i < slices * k; i += nt) list[i] = a.lists[r * slices * k + i];
-		__syncthreads();
+		const uint64_t bound = all_reach > one_reaches ? all_reach : one_reaches;
 		for (int i = tid; i < slices * k; i += nt) {
-			const uint64_t alt = list[i];
-			const int own = i / k;
-			int rank = i - own * k;
-			if (alt == 0u) continue;
-			for (int o = 0; o < slices && rank < k; o++) {
-				if (o == own) continue;
-				const uint64_t * other = list + o * k;
-				int from = 0, to = k;
-				while (from < to) {
-					const int mid = (from + to) >> 1;
-					if (other[mid] > alt) from = mid + 1;
-					else to = mid;
-				}
-				rank += from;
-			}
-			if (rank < k) {
-				a.top_ids[r * k + rank] = score_alternative_id(alt);
-				a.top_logprobs[r * k + rank] = st.log_p(score_alternative_value(alt), a.s);
-			}
+			const uint64_t alt = lists[i];
+			if (alt != 0u && alt >= bound) list[atomicAdd(&count, 1u)] = alt;
 		}
+		__syncthreads();
+		score_rank(list, (int) count, [&](int rank, uint64_t alt) {
+			if (rank >= k) return;
+			a.top_ids[r * k + rank] = score_alternative_id(alt);
+			a.top_logprobs[r * k + rank] = st.log_p(score_alternative_value(alt), a.s);
+		});
+		__syncthreads();
 	}
 }
 
@@ -332,7 +355,7 @@ __device__ __forceinline__ void token_logprobs_join(const LogprobsArgs & a) {
 		TOKEN_LOGPROBS_PACK                                                                                                      \
 		token_logprobs_run<T>(a);                                                                                                \
 	}                                                                                                                            \
-	extern "C" __global__ void __launch_bounds__(SCORE_THREADS) token_logprobs_##SUF##_kernel_finish(TOKEN_LOGPROBS_ARGS(T)) {   \
+	extern "C" __global__ void __launch_bounds__(SCORE_JOIN_THREADS) token_logprobs_##SUF##_kernel_finish(TOKEN_LOGPROBS_ARGS(T)) {   \
 		TOKEN_LOGPROBS_PACK                                                                                                      \
 		token_logprobs_join<T>(a);                                                                                               \
 	}
