@@ -127,6 +127,7 @@ int token_logprobs_set_launch_config(Hip_Launch_Config * hip_launch_config, Data
 	if (score_check_workspace(what, score_logprobs_workspace(n_rows, n_cols, (int) elem, top_k), ARG(op, 13, uint64_t), ARG(op, 14, void *))) return -1;
 	const Score_Plan plan = score_stream_plan(n_rows, n_cols, (int) elem);
 	plan_config(hip_launch_config, plan, n_rows, top_k > 0 ? score_top_lds(plan.waves) : 0);
+	if (top_k > 0) hip_launch_config->variant = HIP_VARIANT_TOP;
 	return 0;
 }
 

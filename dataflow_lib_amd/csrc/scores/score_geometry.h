@@ -30,7 +30,7 @@
 /* Streaming kernels: a row is cut into slices of whole 16-byte chunks (the
  * last one takes the elements behind the last whole chunk too), a workgroup
  * per slice, whose threads take SCORE_BATCH chunks at a time. */
-#define SCORE_BATCH 8   /* twice what score_stream begins its rest with */
+#define SCORE_BATCH 4
 #define SCORE_STREAM_WAVES 8
 #define SCORE_MAP_BATCH 2
 /* few rows: slices until the chip has this many waves */
@@ -126,6 +126,7 @@ GEOM_FN unsigned long score_distill_workspace(int n_rows, int n_cols, int elem_b
  * group maxima (SCORE_GROUP_SLOTS per thread) and which of them reach a bound. */
 #define SCORE_GROUP_SLOTS 4
 #define SCORE_CANDIDATES 1024
+#define SCORE_FEW_COLUMNS 256   /* all of them are candidates */
 GEOM_FN unsigned score_top_lds(int waves) {
 	return (unsigned) (waves * 64 * SCORE_GROUP_SLOTS * 6 + SCORE_CANDIDATES * 8);
 }

@@ -230,7 +230,7 @@ __device__ __forceinline__ RowPart score_stream(const T * row, const RowSlice & 
 		}
 		else {
 			m = -__builtin_inff();
-			if (c + 4 * nt <= sl.last) { m = fmaxf(m, score_chunks<T, 4, ENTROPY>(row, c, s_log2e, p)); c += 4 * nt; }
+			if (SCORE_BATCH > 4 && c + 4 * nt <= sl.last) { m = fmaxf(m, score_chunks<T, 4, ENTROPY>(row, c, s_log2e, p)); c += 4 * nt; }
 			if (c + 2 * nt <= sl.last) { m = fmaxf(m, score_chunks<T, 2, ENTROPY>(row, c, s_log2e, p)); c += 2 * nt; }
 			if (c + nt <= sl.last) { m = fmaxf(m, score_chunks<T, 1, ENTROPY>(row, c, s_log2e, p)); c += nt; }
 			if (c + tid < sl.last) m = fmaxf(m, score_chunks<T, 1, ENTROPY>(row, c, s_log2e, p));
@@ -275,7 +275,7 @@ __device__ __forceinline__ void score_map(const T * row, T * out, const RowSlice
 	const int nt = (int) blockDim.x, tid = (int) threadIdx.x;
 	int c = sl.first;
 	for (; c + SCORE_BATCH * nt <= sl.last; c += SCORE_BATCH * nt) score_map_chunks<T, SCORE_BATCH>(row, out, c, f);
-	if (c + 4 * nt <= sl.last) { score_map_chunks<T, 4>(row, out, c, f); c += 4 * nt; }
+	if (SCORE_BATCH > 4 && c + 4 * nt <= sl.last) { score_map_chunks<T, 4>(row, out, c, f); c += 4 * nt; }
 	if (c + 2 * nt <= sl.last) { score_map_chunks<T, 2>(row, out, c, f); c += 2 * nt; }
 	if (c + nt <= sl.last) { score_map_chunks<T, 1>(row, out, c, f); c += nt; }
 	if (c + tid < sl.last) score_map_chunks<T, 1>(row, out, c, f);

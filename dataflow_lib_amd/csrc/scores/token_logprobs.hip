@@ -31,6 +31,7 @@ __device__ __forceinline__ uint32_t score_group_count(uint32_t n, TopState & t, 
 	if ((threadIdx.x & 63) == 0) cells[threadIdx.x >> 6] = n;
 	__syncthreads();
 	n = 0;
+#pragma unroll 1
 	for (int w = 0; w < waves; w++) n += cells[w];
 	return n;
 }
@@ -41,6 +42,7 @@ template <typename T>
 __device__ __forceinline__ uint32_t score_equal(const T * row, int first, int end, uint32_t key, uint32_t most, uint64_t * list, TopState & t) {
 	const int tid = (int) threadIdx.x, nt = (int) blockDim.x, lane = tid & 63, wave = tid >> 6, waves = nt >> 6;
 	uint32_t have = 0;
+#pragma unroll 1
 	for (long base = first; base < end && have < most; base += nt) {
 		const long j = base + tid;
 		const bool is = j < end && score_key(to_f(row[j < end ? j : first])) == key;
@@ -49,6 +51,7 @@ __device__ __forceinline__ uint32_t score_equal(const T * row, int first, int en
 		if (lane == 0) t.counts[wave] = (uint32_t) __popcll(ballot);
 		__syncthreads();
 		uint32_t before = have + (uint32_t) __popcll(ballot & ((1ull << lane) - 1ull));
+#pragma unroll 1
 		for (int w = 0; w < waves; w++) {
 			if (w < wave) before += t.counts[w];
 			have += t.counts[w];
@@ -67,11 +70,14 @@ __device__ __forceinline__ void score_select(const T * row, int first, int end, 
 	const int tid = (int) threadIdx.x, nt = (int) blockDim.x;
 	__syncthreads();
 	if (tid == 0) { t.prefix = 0u; t.need = (uint32_t) k; t.count = 0u; }
+#pragma unroll 1
 	for (int shift = 24; shift >= 0; shift -= 8) {
+#pragma unroll 1
 		for (int b = tid; b < 256; b += nt) t.hist[b] = 0u;
 		__syncthreads();
 		const uint32_t prefix = t.prefix;
 		const uint32_t above = shift == 24 ? 0u : 0xffffffffu << (shift + 8);
+#pragma unroll 1
 		for (long j = first + tid; j < end; j += nt) {
 			const uint32_t key = score_key(to_f(row[j]));
 			if ((key & above) == prefix) atomicAdd(&t.hist[(key >> shift) & 255u], 1u);
@@ -80,6 +86,7 @@ __device__ __forceinline__ void score_select(const T * row, int first, int end, 
 		if (tid == 0) {
 			uint32_t need = t.need;
 			int b = 255;
+#pragma unroll 1
 			while (b > 0 && t.hist[b] < need) need -= t.hist[b--];
 			t.prefix = prefix | ((uint32_t) b << shift);
 			t.need = need;
@@ -87,6 +94,7 @@ __device__ __forceinline__ void score_select(const T * row, int first, int end, 
 		__syncthreads();
 	}
 	const uint32_t last = t.prefix, equal = t.need;
+#pragma unroll 1
 	for (long j = first + tid; j < end; j += nt) {
 		const uint32_t key = score_key(to_f(row[j]));
 		if (key > last) list[atomicAdd(&t.count, 1u)] = score_alternative(key, (uint32_t) j);
@@ -105,8 +113,9 @@ __device__ __forceinline__ int score_candidates(const T * row, const RowSlice & 
 	const int batches = (sl.last - sl.first + SCORE_BATCH * nt - 1) / (SCORE_BATCH * nt);
 	const int col0 = sl.first * V, col1 = sl.last * V + (sl.end - sl.tail);
 	const bool tail = sl.tail + tid < sl.end;
-	if (sl.columns(V) <= SCORE_CANDIDATES) {
+	if (sl.columns(V) <= SCORE_FEW_COLUMNS) {
 		__syncthreads();
+#pragma unroll 1
 		for (int c = sl.first + tid; c < sl.last; c += nt) {
 			R16 x = score_load(row, (uint64_t) c, 0u);
 			float f[V];
@@ -137,6 +146,7 @@ __device__ __forceinline__ int score_candidates(const T * row, const RowSlice & 
 		 * other bound is interpolated there; the others halve the interval. */
 		float hi = row_max, at_hi = 0.0f;
 		const float aim = __builtin_amdgcn_logf(1.25f * (float) k + 2.0f);
+#pragma unroll 1
 		for (int step = 0; step < 24 && reach > (uint32_t) (k + (k >> 1) + 8); step++) {
 			const float at_lo = __builtin_amdgcn_logf((float) reach);
 			float part = 0.5f;
@@ -198,12 +208,12 @@ __device__ __forceinline__ int score_candidates(const T * row, const RowSlice & 
 		return k;
 	}
 	if (n < k) {
-		/* then columns of -inf, and then those of NaN */
+		/* then columns of -inf, and then those of NaN; a slice may have fewer than k */
 		uint32_t have = (uint32_t) n;
 		have += score_equal(row, col0, col1, score_key(-__builtin_inff()), (uint32_t) k - have, list + have, t);
-		if (have < (uint32_t) k) score_equal(row, col0, col1, 0u, (uint32_t) k - have, list + have, t);
+		if (have < (uint32_t) k) have += score_equal(row, col0, col1, 0u, (uint32_t) k - have, list + have, t);
 		__syncthreads();
-		return k;
+		return (int) have;
 	}
 	return n;
 }
@@ -213,10 +223,11 @@ __device__ __forceinline__ int score_candidates(const T * row, const RowSlice & 
  * number) is called by one of them. */
 template <typename Put>
 __device__ __forceinline__ void score_rank(const uint64_t * list, int n, const Put & put) {
+#pragma unroll 1
 	for (int i = (int) threadIdx.x >> 2; i < n; i += (int) (blockDim.x >> 2)) {
 		const uint64_t alt = list[i];
 		int r = 0;
-#pragma unroll 4
+#pragma unroll 2
 		for (int o = (int) threadIdx.x & 3; o < n; o += 4) r += list[o] > alt ? 1 : 0;
 		r += __builtin_amdgcn_update_dpp(0, r, DPP_QUAD_1032, 0xf, 0xf, false);
 		r += __builtin_amdgcn_update_dpp(0, r, DPP_QUAD_2301, 0xf, 0xf, false);
@@ -245,13 +256,14 @@ __device__ __forceinline__ void token_logprobs_row(const LogprobsArgs & a, long 
 		if (a.entropy) a.entropy[r] = st.entropy();
 		if (a.lse) a.lse[r] = st.lse(a.s);
 	}
+#pragma unroll 1
 	for (int m = (int) threadIdx.x; m < a.tokens_per_row; m += (int) blockDim.x) {
 		const uint32_t t = a.tokens[r * a.tokens_per_row + m];
 		a.logprobs[r * a.tokens_per_row + m] = t < (uint32_t) a.n_cols ? st.log_p(to_f(row[t]), a.s) : 0.0f;
 	}
 }
 
-template <typename T>
+template <typename T, bool TOP>
 __device__ __forceinline__ void token_logprobs_run(const LogprobsArgs & a) {
 	constexpr int V = VecOf<T>::N;
 	__shared__ TopState t;
@@ -261,17 +273,18 @@ __device__ __forceinline__ void token_logprobs_run(const LogprobsArgs & a) {
 	const Score_Plan plan = score_stream_plan(a.n_rows, a.n_cols, (int) sizeof(T));
 	const int tid = (int) threadIdx.x, nt = (int) blockDim.x;
 	const float s_log2e = a.s * SCORE_LOG2E;
+#pragma unroll 1
 	for (long w = blockIdx.x; w < (long) a.n_rows * plan.slices; w += gridDim.x) {
 		const long r = plan.slices == 1 ? w : w / plan.slices;
 		const int slice = plan.slices == 1 ? 0 : (int) (w - r * plan.slices);
 		const T * row = static_cast<const T *>(a.logits) + (uint64_t) r * a.row_stride;
 		const RowSlice sl(a.n_cols, V, slice, plan.slices, plan.slice_chunks);
-		RowPart p = score_stream<T, true>(row, sl, s_log2e, a.top_k > 0 ? groups : nullptr);
+		RowPart p = score_stream<T, true>(row, sl, s_log2e, TOP ? groups : nullptr);
 		p = score_group_join(p, s_log2e, t.cells);
 		const RowStats st(p.m, p.z, p.e);
 		if (plan.slices == 1) token_logprobs_row<T>(a, r, row, st);
 		else if (tid == 0) a.parts[w] = Score_Part{p.m, p.z, p.e, 0.0f};
-		if (a.top_k > 0) {
+		if (TOP) {
 			const int k = a.top_k;
 			const int n = score_candidates(row, sl, k, p.m, groups, reached, list, t);
 			score_rank(list, n, [&](int rank, uint64_t alt) {
@@ -351,9 +364,13 @@ __device__ __forceinline__ void token_logprobs_join(const LogprobsArgs & a) {
 	a.lists = static_cast<uint64_t *>(workspace);                                                                                \
 	a.parts = reinterpret_cast<Score_Part *>(a.lists + (uint64_t) n_rows * plan.slices * top_k);
 #define TOKEN_LOGPROBS_KERNEL(SUF, T)                                                                                            \
-	extern "C" __global__ void __launch_bounds__(64 * SCORE_STREAM_WAVES, 2) token_logprobs_##SUF##_kernel(TOKEN_LOGPROBS_ARGS(T)) { \
+	extern "C" __global__ void __launch_bounds__(64 * SCORE_STREAM_WAVES, 8) token_logprobs_##SUF##_kernel(TOKEN_LOGPROBS_ARGS(T)) { \
 		TOKEN_LOGPROBS_PACK                                                                                                      \
-		token_logprobs_run<T>(a);                                                                                                \
+		token_logprobs_run<T, false>(a);                                                                                                \
+	}                                                                                                                            \
+	extern "C" __global__ void __launch_bounds__(64 * SCORE_STREAM_WAVES, 8) token_logprobs_##SUF##_kernel_top(TOKEN_LOGPROBS_ARGS(T)) { \
+		TOKEN_LOGPROBS_PACK                                                                                                      \
+		token_logprobs_run<T, true>(a);                                                                                          \
 	}                                                                                                                            \
 	extern "C" __global__ void __launch_bounds__(SCORE_JOIN_THREADS) token_logprobs_##SUF##_kernel_finish(TOKEN_LOGPROBS_ARGS(T)) {   \
 		TOKEN_LOGPROBS_PACK                                                                                                      \

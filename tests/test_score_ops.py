@@ -191,8 +191,8 @@ def to_storage_like(dt, shape):
 class HipFunction(ctypes.Structure):
     """Hip_Function (hip_dataflow_handle.h)"""
     _fields_ = [("func_max_smem", ctypes.c_int), ("func_max_threads_per_block", ctypes.c_int), ("shares_module_scratch", ctypes.c_int),
-                ("occupancy_memo", ctypes.c_uint64 * 8), ("is_native", ctypes.c_bool), ("function_handle", ctypes.c_void_p),
-                ("set_launch_config", ctypes.c_void_p), ("finish_function_handle", ctypes.c_void_p), ("variant_handles", ctypes.c_void_p * 7),
+                ("occupancy_memo", ctypes.c_uint64 * 9), ("is_native", ctypes.c_bool), ("function_handle", ctypes.c_void_p),
+                ("set_launch_config", ctypes.c_void_p), ("finish_function_handle", ctypes.c_void_p), ("variant_handles", ctypes.c_void_p * 8),
                 ("set_finish_launch_config", ctypes.c_void_p), ("hip_external_func", ctypes.c_void_p), ("op_extra", ctypes.c_void_p),
                 ("op_skeleton", api.OpSkeleton)]
 
