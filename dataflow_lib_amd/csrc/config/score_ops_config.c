@@ -125,7 +125,7 @@ int token_logprobs_set_launch_config(Hip_Launch_Config * hip_launch_config, Data
 	if (top_k > 0 && (score_pointer(what, "the top id pointer", ARG(op, 11, void *), 4) ||
 					  score_pointer(what, "the top log-probability pointer", ARG(op, 12, void *), 4))) return -1;
 	if (score_check_workspace(what, score_logprobs_workspace(n_rows, n_cols, (int) elem, top_k), ARG(op, 13, uint64_t), ARG(op, 14, void *))) return -1;
-	const Score_Plan plan = score_stream_plan(n_rows, n_cols, (int) elem);
+	const Score_Plan plan = score_stream_plan(n_rows, n_cols, (int) elem, top_k);
 	plan_config(hip_launch_config, plan, n_rows, top_k > 0 ? score_top_lds(plan.waves) : 0);
 	if (top_k > 0) hip_launch_config->variant = HIP_VARIANT_TOP;
 	return 0;
@@ -135,7 +135,7 @@ int token_logprobs_set_launch_config(Hip_Launch_Config * hip_launch_config, Data
 int token_logprobs_set_finish_launch_config(Hip_Launch_Config * hip_launch_config, Dataflow_Handle * dataflow_handle, Hip_Function * hip_function, Op * op) {
 	(void) dataflow_handle;
 	const int n_rows = ARG(op, 0, int), top_k = ARG(op, 5, int);
-	const Score_Plan plan = score_stream_plan(n_rows, ARG(op, 1, int), (int) logits_elem(hip_function));
+	const Score_Plan plan = score_stream_plan(n_rows, ARG(op, 1, int), (int) logits_elem(hip_function), top_k);
 	set_1d(hip_launch_config, plan.slices > 1 ? (unsigned) n_rows : 0u, SCORE_JOIN_THREADS, (unsigned) (8 * plan.slices * top_k));
 	return 0;
 }
@@ -196,7 +196,7 @@ int distillation_loss_set_launch_config(Hip_Launch_Config * hip_launch_config, D
 		hip_launch_config->variant = variant;
 		return 0;
 	}
-	const Score_Plan plan = score_stream_plan(n_rows, n_cols, (int) elem);
+	const Score_Plan plan = score_stream_plan(n_rows, n_cols, (int) elem, 0);
 	plan_config(hip_launch_config, plan, n_rows, 0);
 	if (plan.slices > 1 || ARG(op, 12, void *)) hip_launch_config->then_variant = HIP_VARIANT_SPLIT_OUT;
 	return 0;
@@ -206,6 +206,6 @@ int distillation_loss_set_launch_config(Hip_Launch_Config * hip_launch_config, D
 int distillation_loss_set_finish_launch_config(Hip_Launch_Config * hip_launch_config, Dataflow_Handle * dataflow_handle, Hip_Function * hip_function, Op * op) {
 	(void) dataflow_handle;
 	(void) hip_function;
-	set_1d(hip_launch_config, ARG(op, 11, void *) ? 1u : 0u, SCORE_THREADS, 0);
+	set_1d(hip_launch_config, ARG(op, 11, void *) ? 1u : 0u, SCORE_MEAN_THREADS, 0);
 	return 0;
 }

@@ -51,27 +51,6 @@ struct DistillCells {
 	float m[SCORE_MAX_WAVES], z[SCORE_MAX_WAVES], vm[SCORE_MAX_WAVES], vz[SCORE_MAX_WAVES], loss[SCORE_MAX_WAVES];
 };
 
-/* a row's parts, one per wave, joined by the lanes of each wave alike: lane i
- * takes cell i of 16, and all rows of 16 lanes end with the total */
-__device__ __forceinline__ RowPart join_cells(const float * m, const float * z, int waves, float s_log2e) {
-	const int i = (int) threadIdx.x & 15;
-	RowPart p;
-	p.m = i < waves ? m[i] : -__builtin_inff();
-	p.z = i < waves ? z[i] : 0.0f;
-	float t = fmaxf(p.m, dpp_f32<DPP_QUAD_1032>(p.m));
-	t = fmaxf(t, dpp_f32<DPP_QUAD_2301>(t));
-	t = fmaxf(t, dpp_f32<DPP_ROW_HALF_MIRROR>(t));
-	t = fmaxf(t, dpp_f32<DPP_ROW_MIRROR>(t));
-	p.shift(t, s_log2e);
-	p.z += dpp_f32<DPP_QUAD_1032>(p.z);
-	p.z += dpp_f32<DPP_QUAD_2301>(p.z);
-	p.z += dpp_f32<DPP_ROW_HALF_MIRROR>(p.z);
-	p.z += dpp_f32<DPP_ROW_MIRROR>(p.z);
-	p.m = readlane_f32(p.m, 0);
-	p.z = readlane_f32(p.z, 0);
-	return p;
-}
-
 template <typename T> __device__ __forceinline__ float buf_load_elem(__amdgpu_buffer_rsrc_t r, uint32_t off);
 template <> __device__ __forceinline__ float buf_load_elem<float>(__amdgpu_buffer_rsrc_t r, uint32_t off) {
 	return __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(r, off, 0, 0));
@@ -214,9 +193,9 @@ __device__ __forceinline__ void distill_held(const DistillArgs & a) {
 				a.loss[before] = l * temperature * temperature;
 			}
 		}
-		p = join_cells(cells.m, cells.z, waves, s_log2e);
+		p = score_join_cells(cells.m, cells.z, nullptr, waves, s_log2e);
 		const int teacher_waves = K == 0 ? 0 : (K + 63) >> 6;
-		te = join_cells(cells.vm, cells.vz, teacher_waves, s_log2e);
+		te = score_join_cells(cells.vm, cells.vz, nullptr, teacher_waves, s_log2e);
 		const RowStats st(p.m, p.z, 0.0f);
 		const bool counts = w != 0.0f && !(te.z == 0.0f);
 		const float wt = w * temperature;
@@ -312,7 +291,7 @@ __device__ __forceinline__ bool distill_teacher(const DistillArgs & a, long r, c
 		sum.shift(m, a.s * SCORE_LOG2E);
 		sum.z += is ? one.z * __builtin_amdgcn_exp2f(fmaxf((one.m - m) * a.s * SCORE_LOG2E, SCORE_FAR_BELOW)) : 0.0f;
 	}
-	sum = score_group_join(sum, a.s * SCORE_LOG2E, cells);
+	sum = score_group_join<false>(sum, a.s * SCORE_LOG2E, cells);
 	if (sum.z == 0.0f) {
 		if (threadIdx.x == 0 && write_loss) a.loss[r] = 0.0f;
 		return false;
@@ -340,7 +319,7 @@ template <typename T>
 __device__ __forceinline__ void distill_parts(const DistillArgs & a) {
 	__shared__ float cells[3 * SCORE_MAX_WAVES];
 	__shared__ Teacher te;
-	const Score_Plan plan = score_stream_plan(a.n_rows, a.n_cols, (int) sizeof(T));
+	const Score_Plan plan = score_stream_plan(a.n_rows, a.n_cols, (int) sizeof(T), 0);
 	const float s_log2e = a.s * SCORE_LOG2E;
 	for (long u = blockIdx.x; u < (long) a.n_rows * plan.slices; u += gridDim.x) {
 		const long r = plan.slices == 1 ? u : u / plan.slices;
@@ -352,7 +331,7 @@ __device__ __forceinline__ void distill_parts(const DistillArgs & a) {
 			continue;
 		}
 		const RowSlice sl(a.n_cols, VecOf<T>::N, slice, plan.slices, plan.slice_chunks);
-		const RowPart p = score_group_join(score_stream<T, false>(row, sl, s_log2e, nullptr), s_log2e, cells);
+		const RowPart p = score_group_join<false>(score_stream<T, false, false>(row, sl, s_log2e, nullptr), s_log2e, cells);
 		if (alone) {
 			distill_teacher(a, r, RowStats(p.m, p.z, 0.0f), true, te, cells, [&](int, uint32_t id) { return to_f(row[id]); });
 			continue;
@@ -373,7 +352,7 @@ template <typename T>
 __device__ __forceinline__ void distill_out(const DistillArgs & a) {
 	__shared__ float cells[3 * SCORE_MAX_WAVES];
 	__shared__ Teacher te;
-	const Score_Plan plan = score_stream_plan(a.n_rows, a.n_cols, (int) sizeof(T));
+	const Score_Plan plan = score_stream_plan(a.n_rows, a.n_cols, (int) sizeof(T), 0);
 	const float s_log2e = a.s * SCORE_LOG2E, temperature = 1.0f / a.s;
 	for (long u = blockIdx.x; u < (long) a.n_rows * plan.slices; u += gridDim.x) {
 		const long r = plan.slices == 1 ? u : u / plan.slices;
@@ -425,18 +404,21 @@ __device__ __forceinline__ void distill_out(const DistillArgs & a) {
 
 /* mean_loss = sum_r w_r loss_r / n_rows in 64 bits, in a fixed order */
 __device__ __forceinline__ void distillation_loss_mean(int n_rows, const float * row_weights, const float * loss, float * mean_loss) {
-	__shared__ double part[SCORE_THREADS];
+	__shared__ double part[SCORE_MAX_WAVES];
 	double sum = 0.0;
-	for (long r = threadIdx.x; r < n_rows; r += blockDim.x) {
-		const float w = row_weights ? row_weights[r] : 1.0f;
-		if (w != 0.0f) sum += (double) w * (double) loss[r];
+#pragma unroll 4
+	for (long r = threadIdx.x; r < n_rows; r += SCORE_MEAN_THREADS) {
+		const float w = row_weights ? row_weights[r] : 1.0f, l = loss[r];
+		sum += w != 0.0f ? (double) w * (double) l : 0.0;
 	}
-	part[threadIdx.x] = sum;
-	for (int step = SCORE_THREADS / 2; step > 0; step /= 2) {
-		__syncthreads();
-		if ((int) threadIdx.x < step) part[threadIdx.x] += part[threadIdx.x + step];
+	for (int step = 32; step > 0; step >>= 1) sum += __shfl_xor(sum, step);
+	if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = sum;
+	__syncthreads();
+	if (threadIdx.x == 0) {
+		sum = 0.0;
+		for (int i = 0; i < SCORE_MEAN_THREADS / 64; i++) sum += part[i];
+		*mean_loss = (float) (sum / (double) n_rows);
 	}
-	if (threadIdx.x == 0) *mean_loss = (float) (part[0] / (double) n_rows);
 }
 
 #define DISTILLATION_ARGS(T)                                                                                                     \
@@ -446,7 +428,7 @@ __device__ __forceinline__ void distillation_loss_mean(int n_rows, const float *
 #define DISTILLATION_PACK                                                                                                        \
 	DistillArgs a = {n_rows, n_cols, row_stride, grad_stride, scale, top_k, logits, teacher_ids, teacher_logits, row_weights,    \
 					 loss, dlogits, static_cast<Score_Part *>(workspace), nullptr};                                              \
-	a.picked = reinterpret_cast<float *>(a.parts + (uint64_t) n_rows * score_stream_plan(n_rows, n_cols, (int) sizeof(*logits)).slices);
+	a.picked = reinterpret_cast<float *>(a.parts + (uint64_t) n_rows * score_stream_plan(n_rows, n_cols, (int) sizeof(*logits), 0).slices);
 #define DISTILLATION_LOSS_KERNEL(SUF, T)                                                                                         \
 	extern "C" __global__ void __launch_bounds__(1024) distillation_loss_##SUF##_kernel_long_rows(DISTILLATION_ARGS(T)) { \
 		DISTILLATION_PACK \
@@ -460,15 +442,15 @@ __device__ __forceinline__ void distillation_loss_mean(int n_rows, const float *
 		DISTILLATION_PACK \
 		distill_held<T, SCORE_HELD, 0>(a); \
 	} \
-	extern "C" __global__ void __launch_bounds__(64 * SCORE_STREAM_WAVES) distillation_loss_##SUF##_kernel(DISTILLATION_ARGS(T)) { \
+	extern "C" __global__ void __launch_bounds__(64 * SCORE_MAX_WAVES, 8) distillation_loss_##SUF##_kernel(DISTILLATION_ARGS(T)) { \
 		DISTILLATION_PACK                                                                                                        \
 		distill_parts<T>(a);                                                                                                     \
 	}                                                                                                                            \
-	extern "C" __global__ void __launch_bounds__(64 * SCORE_STREAM_WAVES) distillation_loss_##SUF##_kernel_split_out(DISTILLATION_ARGS(T)) { \
+	extern "C" __global__ void __launch_bounds__(64 * SCORE_MAX_WAVES, 8) distillation_loss_##SUF##_kernel_split_out(DISTILLATION_ARGS(T)) { \
 		DISTILLATION_PACK                                                                                                        \
 		distill_out<T>(a);                                                                                                       \
 	}                                                                                                                            \
-	extern "C" __global__ void __launch_bounds__(SCORE_THREADS) distillation_loss_##SUF##_kernel_finish(DISTILLATION_ARGS(T)) {  \
+	extern "C" __global__ void __launch_bounds__(SCORE_MEAN_THREADS) distillation_loss_##SUF##_kernel_finish(DISTILLATION_ARGS(T)) {  \
 		distillation_loss_mean(n_rows, row_weights, loss, mean_loss);                                                            \
 	}
 

@@ -24,8 +24,7 @@
 /* so many workgroups at most, which walk what is left: every launch stays
  * below 2^32 threads */
 #define SCORE_MAX_GROUPS (1 << 20)
-/* simple row kernels and the mean loss */
-#define SCORE_THREADS 256
+#define SCORE_MEAN_THREADS 1024
 
 /* Streaming kernels: a row is cut into slices of whole 16-byte chunks (the
  * last one takes the elements behind the last whole chunk too), a workgroup
@@ -33,8 +32,12 @@
 #define SCORE_BATCH 4
 #define SCORE_STREAM_WAVES 8
 #define SCORE_MAP_BATCH 2
-/* few rows: slices until the chip has this many waves */
+/* few rows: slices until the chip has this many waves, each of at least
+ * SCORE_SLICE_BATCH chunks per thread. Fewer than SCORE_MIN_SLICES are not worth
+ * the second launch that joins them. */
 #define SCORE_FILL_WAVES 2048
+#define SCORE_SLICE_BATCH 4
+#define SCORE_MIN_SLICES 3
 #define SCORE_MAX_SLICES 32   /* fewer than a wave's lanes, one of which joins each */
 #define SCORE_JOIN_THREADS 512
 
@@ -46,28 +49,33 @@ typedef struct {
 } Score_Plan;
 
 /* waves that a row fills with `batch` chunks per thread, at most max_waves of
- * them to a workgroup; few rows are cut into slices of whole such workgroups
- * until the chip has SCORE_FILL_WAVES waves */
+ * them to a workgroup; few rows are cut into slices of SCORE_SLICE_BATCH chunks
+ * per thread or more until the chip has SCORE_FILL_WAVES waves */
 GEOM_FN Score_Plan score_plan(int n_rows, int n_cols, int elem_bytes, int batch, int max_waves) {
 	Score_Plan p;
 	const long chunks = (long) n_cols * elem_bytes / 16;
-	const long per_wave = 64 * batch;
-	long waves = (chunks + per_wave - 1) / per_wave;
+	long waves = (chunks + 64 * batch - 1) / (64 * batch);
 	if (waves < 1) waves = 1;
 	p.waves = (int) (waves < max_waves ? waves : max_waves);
 	p.slices = 1;
-	const long most = waves / max_waves;
+	const long most = chunks / (64 * SCORE_SLICE_BATCH * max_waves);
 	long want = SCORE_FILL_WAVES / ((long) n_rows * p.waves);
 	if (want > most) want = most;
 	if (want > SCORE_MAX_SLICES) want = SCORE_MAX_SLICES;
-	if (want > 1) p.slices = (int) want;
+	if (want >= SCORE_MIN_SLICES) p.slices = (int) want;
 	p.slice_chunks = (int) ((chunks + p.slices - 1) / p.slices);
 	if (p.slices > 1) p.slices = (int) ((chunks + p.slice_chunks - 1) / p.slice_chunks);
 	return p;
 }
 
-GEOM_FN Score_Plan score_stream_plan(int n_rows, int n_cols, int elem_bytes) {
-	return score_plan(n_rows, n_cols, elem_bytes, SCORE_BATCH, SCORE_STREAM_WAVES);
+/* token_logprobs and the statistics of distillation_loss. Where no alternatives
+ * are to be found, rows in one slice that would leave half of the chip's waves
+ * free take workgroups of twice as many. */
+GEOM_FN Score_Plan score_stream_plan(int n_rows, int n_cols, int elem_bytes, int top_k) {
+	Score_Plan p = score_plan(n_rows, n_cols, elem_bytes, SCORE_BATCH, SCORE_STREAM_WAVES);
+	if (top_k == 0 && p.slices == 1 && (long) n_rows * SCORE_STREAM_WAVES <= 2 * SCORE_FILL_WAVES && p.slice_chunks >= 64 * 4 * SCORE_STREAM_WAVES)
+		p.waves = 2 * SCORE_STREAM_WAVES;
+	return p;
 }
 
 /* the gradient kernels, which read and write a row once */
@@ -84,7 +92,7 @@ typedef struct {
 
 GEOM_FN unsigned long score_logprobs_workspace(int n_rows, int n_cols, int elem_bytes, int top_k) {
 	if (n_rows <= 0 || n_cols <= 0 || elem_bytes <= 0 || top_k < 0) return 0;
-	const Score_Plan p = score_stream_plan(n_rows, n_cols, elem_bytes);
+	const Score_Plan p = score_stream_plan(n_rows, n_cols, elem_bytes, top_k);
 	if (p.slices == 1) return 0;
 	return (unsigned long) n_rows * (unsigned long) p.slices * (sizeof(Score_Part) + 8ul * (unsigned long) top_k);
 }
@@ -117,7 +125,7 @@ GEOM_FN int score_held_waves(int held, int n_cols, int elem_bytes, int top_k) {
 /* a call may want the loss alone, whatever its sizes */
 GEOM_FN unsigned long score_distill_workspace(int n_rows, int n_cols, int elem_bytes, int top_k) {
 	if (n_rows <= 0 || n_cols <= 0 || elem_bytes <= 0 || top_k < 0) return 0;
-	const Score_Plan p = score_stream_plan(n_rows, n_cols, elem_bytes);
+	const Score_Plan p = score_stream_plan(n_rows, n_cols, elem_bytes, 0);
 	if (p.slices == 1 && score_held(n_rows, n_cols, elem_bytes, top_k)) return 0;
 	return (unsigned long) n_rows * ((unsigned long) p.slices * sizeof(Score_Part) + 4ul * (unsigned long) top_k);
 }

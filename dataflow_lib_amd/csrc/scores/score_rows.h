@@ -62,65 +62,103 @@ struct RowPart {
 	}
 };
 
-/* sums and maxima over a workgroup; `cells`: SCORE_MAX_WAVES floats of LDS */
+/* What a workgroup's waves have left in one cell each, joined by the lanes of
+ * every wave alike: lane i takes cell i (of SCORE_MAX_WAVES, as many as a row
+ * of lanes for the DPP steps), one LDS access for all of them. */
+template <typename Op>
+__device__ __forceinline__ float score_row16(float v, const Op & op) {
+	v = op(v, dpp_f32<DPP_QUAD_1032>(v));
+	v = op(v, dpp_f32<DPP_QUAD_2301>(v));
+	v = op(v, dpp_f32<DPP_ROW_HALF_MIRROR>(v));
+	return op(v, dpp_f32<DPP_ROW_MIRROR>(v));
+}
+struct ScoreMax { __device__ __forceinline__ float operator()(float a, float b) const { return fmaxf(a, b); } };
+struct ScoreSum { __device__ __forceinline__ float operator()(float a, float b) const { return a + b; } };
+template <typename Op>
+__device__ __forceinline__ float score_cells(const float * cells, float none, const Op & op) {
+	const int i = (int) threadIdx.x & (SCORE_MAX_WAVES - 1);
+	return readlane_f32(score_row16(i < (int) (blockDim.x >> 6) ? cells[i] : none, op), 0);
+}
+/* maximum or sum over a workgroup; `cells`: SCORE_MAX_WAVES floats of LDS */
 __device__ __forceinline__ float score_group_max(float v, float * cells) {
 	v = wave_max(v);
-	const int waves = (int) (blockDim.x >> 6);
+	if (blockDim.x == 64) return v;
 	__syncthreads();
 	if ((threadIdx.x & 63) == 0) cells[threadIdx.x >> 6] = v;
 	__syncthreads();
-	v = cells[0];
-	for (int w = 1; w < waves; w++) v = fmaxf(v, cells[w]);
-	return v;
+	return score_cells(cells, -__builtin_inff(), ScoreMax());
 }
 __device__ __forceinline__ float score_group_sum(float v, float * cells) {
 	v = wave_sum(v);
-	const int waves = (int) (blockDim.x >> 6);
+	if (blockDim.x == 64) return v;
 	__syncthreads();
 	if ((threadIdx.x & 63) == 0) cells[threadIdx.x >> 6] = v;
 	__syncthreads();
-	v = cells[0];
-	for (int w = 1; w < waves; w++) v += cells[w];
-	return v;
+	return score_cells(cells, 0.0f, ScoreSum());
+}
+/* parts of a row, one per wave: maxima, and sums shifted by them */
+__device__ __forceinline__ RowPart score_join_cells(const float * m, const float * z, const float * e, int waves, float s_log2e) {
+	const int i = (int) threadIdx.x & (SCORE_MAX_WAVES - 1);
+	RowPart p;
+	if (i < waves) {
+		p.m = m[i];
+		p.z = z[i];
+		if (e) p.e = e[i];
+	}
+	p.shift(score_row16(p.m, ScoreMax()), s_log2e);
+	p.z = readlane_f32(score_row16(p.z, ScoreSum()), 0);
+	if (e) p.e = readlane_f32(score_row16(p.e, ScoreSum()), 0);
+	p.m = readlane_f32(p.m, 0);
+	return p;
 }
 /* the parts of a workgroup's threads, joined (every thread gets the result);
- * `cells`: 3 SCORE_MAX_WAVES floats of LDS */
-__device__ __forceinline__ RowPart score_group_join(RowPart p, float s_log2e, float * cells) {
+ * `cells`: 5 SCORE_MAX_WAVES floats of LDS. With TOP also the threads that have
+ * met a column above -inf: how many, and the least of their maxima. */
+template <bool TOP>
+__device__ __forceinline__ RowPart score_group_join(RowPart p, float s_log2e, float * cells, float * met = nullptr, float * least = nullptr) {
 	const int wave = (int) (threadIdx.x >> 6), waves = (int) (blockDim.x >> 6);
+	float n = 0.0f, l = 0.0f;
+	if (TOP) {
+		const bool has = p.m > -__builtin_inff();
+		n = (float) __popcll(__ballot(has));
+		l = wave_max(has ? -p.m : -__builtin_inff());
+	}
 	p.shift(wave_max(p.m), s_log2e);
 	p.z = wave_sum(p.z);
 	p.e = wave_sum(p.e);
-	if (waves == 1) return p;
-	__syncthreads();
-	if ((threadIdx.x & 63) == 0) {
-		cells[wave] = p.m;
-		cells[SCORE_MAX_WAVES + wave] = p.z;
-		cells[2 * SCORE_MAX_WAVES + wave] = p.e;
+	if (waves > 1) {
+		__syncthreads();
+		if ((threadIdx.x & 63) == 0) {
+			cells[wave] = p.m;
+			cells[SCORE_MAX_WAVES + wave] = p.z;
+			cells[2 * SCORE_MAX_WAVES + wave] = p.e;
+			if (TOP) {
+				cells[3 * SCORE_MAX_WAVES + wave] = n;
+				cells[4 * SCORE_MAX_WAVES + wave] = l;
+			}
+		}
+		__syncthreads();
+		p = score_join_cells(cells, cells + SCORE_MAX_WAVES, cells + 2 * SCORE_MAX_WAVES, waves, s_log2e);
+		if (TOP) {
+			n = score_cells(cells + 3 * SCORE_MAX_WAVES, 0.0f, ScoreSum());
+			l = score_cells(cells + 4 * SCORE_MAX_WAVES, -__builtin_inff(), ScoreMax());
+		}
 	}
-	__syncthreads();
-	float m = cells[0];
-	for (int w = 1; w < waves; w++) m = fmaxf(m, cells[w]);
-	RowPart sum;
-	sum.m = m;
-	for (int w = 0; w < waves; w++) {
-		RowPart q;
-		q.m = cells[w];
-		q.z = cells[SCORE_MAX_WAVES + w];
-		q.e = cells[2 * SCORE_MAX_WAVES + w];
-		q.shift(m, s_log2e);
-		sum.z += q.z;
-		sum.e += q.e;
+	if (TOP) {
+		*met = n;
+		*least = -l;
 	}
-	return sum;
+	return p;
 }
 
 /* 16 bytes of a row, which need no more alignment than its elements (of two
  * bytes at least) */
 typedef uint32_t score_vec __attribute__((ext_vector_type(4), aligned(2)));
-template <typename T>
+template <typename T, bool AGAIN = false>
 __device__ __forceinline__ R16 score_load(const T * row, uint64_t uniform_chunk, uint32_t lane_chunk) {
-	const char * p = reinterpret_cast<const char *>(row) + uniform_chunk * 16u;
-	const score_vec v = __builtin_nontemporal_load(reinterpret_cast<const score_vec *>(p + lane_chunk * 16u));
+	const score_vec * p = reinterpret_cast<const score_vec *>(reinterpret_cast<const char *>(row) + uniform_chunk * 16u + lane_chunk * 16u);
+	/* read once: with the streaming hint */
+	const score_vec v = AGAIN ? *p : __builtin_nontemporal_load(p);
 	R16 r;
 	r.w[0] = v.x; r.w[1] = v.y; r.w[2] = v.z; r.w[3] = v.w;
 	return r;
@@ -147,12 +185,12 @@ struct RowSlice {
  * maximum, the part's shift to it, then their terms. -inf makes E's term NaN
  * (-inf * 0): a wave that finds NaN in its sum forms the terms again, with
  * exponents that are far below 0 but finite. Returns the chunks' maximum. */
-template <typename T, int N, bool ENTROPY>
+template <typename T, int N, bool ENTROPY, bool AGAIN>
 __device__ __forceinline__ float score_chunks(const T * row, int c, float s_log2e, RowPart & p) {
 	constexpr int V = VecOf<T>::N;
 	R16 x[N];
 #pragma unroll
-	for (int u = 0; u < N; u++) x[u] = score_load(row, (uint64_t) (c + u * (int) blockDim.x), threadIdx.x);
+	for (int u = 0; u < N; u++) x[u] = score_load<T, AGAIN>(row, (uint64_t) (c + u * (int) blockDim.x), threadIdx.x);
 	float m = -__builtin_inff();
 #pragma unroll
 	for (int u = 0; u < N; u++) {
@@ -208,8 +246,8 @@ __device__ __forceinline__ float score_chunks(const T * row, int c, float s_log2
  * in batches of half, a quarter and so on, so that only the last chunk has to
  * ask whether it is there. The maximum of the thread's b-th batch (what is left
  * being one) goes to groups[(b % SCORE_GROUP_SLOTS) * blockDim.x + tid] (LDS;
- * null: not wanted); the element behind the last whole chunk counts to batch 0. */
-template <typename T, bool ENTROPY>
+ * null: not wanted); AGAIN: some chunks are read again soon. The element behind the last whole chunk counts to batch 0. */
+template <typename T, bool ENTROPY, bool AGAIN>
 __device__ __forceinline__ RowPart score_stream(const T * row, const RowSlice & sl, float s_log2e, float * groups) {
 	const int nt = (int) blockDim.x, tid = (int) threadIdx.x;
 	RowPart p;
@@ -225,15 +263,15 @@ __device__ __forceinline__ RowPart score_stream(const T * row, const RowSlice & 
 		float m;
 		const bool whole = c + SCORE_BATCH * nt <= sl.last;
 		if (whole) {
-			m = score_chunks<T, SCORE_BATCH, ENTROPY>(row, c, s_log2e, p);
+			m = score_chunks<T, SCORE_BATCH, ENTROPY, AGAIN>(row, c, s_log2e, p);
 			c += SCORE_BATCH * nt;
 		}
 		else {
 			m = -__builtin_inff();
-			if (SCORE_BATCH > 4 && c + 4 * nt <= sl.last) { m = fmaxf(m, score_chunks<T, 4, ENTROPY>(row, c, s_log2e, p)); c += 4 * nt; }
-			if (c + 2 * nt <= sl.last) { m = fmaxf(m, score_chunks<T, 2, ENTROPY>(row, c, s_log2e, p)); c += 2 * nt; }
-			if (c + nt <= sl.last) { m = fmaxf(m, score_chunks<T, 1, ENTROPY>(row, c, s_log2e, p)); c += nt; }
-			if (c + tid < sl.last) m = fmaxf(m, score_chunks<T, 1, ENTROPY>(row, c, s_log2e, p));
+			if (SCORE_BATCH > 4 && c + 4 * nt <= sl.last) { m = fmaxf(m, score_chunks<T, 4, ENTROPY, AGAIN>(row, c, s_log2e, p)); c += 4 * nt; }
+			if (c + 2 * nt <= sl.last) { m = fmaxf(m, score_chunks<T, 2, ENTROPY, AGAIN>(row, c, s_log2e, p)); c += 2 * nt; }
+			if (c + nt <= sl.last) { m = fmaxf(m, score_chunks<T, 1, ENTROPY, AGAIN>(row, c, s_log2e, p)); c += nt; }
+			if (c + tid < sl.last) m = fmaxf(m, score_chunks<T, 1, ENTROPY, AGAIN>(row, c, s_log2e, p));
 		}
 		if (groups) {
 			float * g = groups + slot * nt + tid;
@@ -294,14 +332,6 @@ __device__ __forceinline__ void score_clear(T * out, const RowSlice & sl) {
 __device__ __forceinline__ void score_stores_done() {
 	__builtin_amdgcn_s_waitcnt(0x0F70);   /* vmcnt(0) */
 	__syncthreads();
-}
-
-template <typename T>
-__device__ __forceinline__ RowStats score_row_stats(const T * row, int n_cols, float s, float * cells) {
-	constexpr int V = VecOf<T>::N;
-	const RowSlice sl(n_cols, V, 0, 1, n_cols / V);
-	const RowPart p = score_group_join(score_stream<T, false>(row, sl, s * SCORE_LOG2E, nullptr), s * SCORE_LOG2E, cells);
-	return RowStats(p.m, p.z, p.e);
 }
 
 /* Whole numbers that lie as floats do: -0 with +0, NaN below -inf. */

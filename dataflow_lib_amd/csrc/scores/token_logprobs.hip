@@ -16,8 +16,8 @@
 #include "score_rows.h"
 
 struct TopState {
-	float cells[3 * SCORE_MAX_WAVES];
-	uint32_t counts[2 * SCORE_MAX_WAVES];
+	float cells[5 * SCORE_MAX_WAVES];
+	float counts[2 * SCORE_MAX_WAVES];
 	uint32_t hist[256];
 	uint32_t prefix, need, count, n_groups;
 };
@@ -25,15 +25,11 @@ struct TopState {
 /* a count over a workgroup of a wave's count; calls alternate between two
  * sets of cells, so one barrier each is enough */
 __device__ __forceinline__ uint32_t score_group_count(uint32_t n, TopState & t, int & turn) {
-	const int waves = (int) (blockDim.x >> 6);
-	if (waves == 1) return n;
-	uint32_t * cells = t.counts + (turn ^= SCORE_MAX_WAVES);
-	if ((threadIdx.x & 63) == 0) cells[threadIdx.x >> 6] = n;
-	__syncthreads();
-	n = 0;
-#pragma unroll 1
-	for (int w = 0; w < waves; w++) n += cells[w];
-	return n;
+	if (blockDim.x == 64) return n;
+	float * cells = t.counts + (turn ^= SCORE_MAX_WAVES);
+	if ((threadIdx.x & 63) == 0) cells[threadIdx.x >> 6] = (float) n;
+	lds_barrier();
+	return (uint32_t) score_cells(cells, 0.0f, ScoreSum());
 }
 
 /* Of the columns [first, end) those whose key is `key`, by rising column, the
@@ -48,13 +44,13 @@ __device__ __forceinline__ uint32_t score_equal(const T * row, int first, int en
 		const bool is = j < end && score_key(to_f(row[j < end ? j : first])) == key;
 		const unsigned long long ballot = __ballot(is);
 		__syncthreads();
-		if (lane == 0) t.counts[wave] = (uint32_t) __popcll(ballot);
+		if (lane == 0) t.counts[wave] = (float) __popcll(ballot);
 		__syncthreads();
 		uint32_t before = have + (uint32_t) __popcll(ballot & ((1ull << lane) - 1ull));
 #pragma unroll 1
 		for (int w = 0; w < waves; w++) {
-			if (w < wave) before += t.counts[w];
-			have += t.counts[w];
+			if (w < wave) before += (uint32_t) t.counts[w];
+			have += (uint32_t) t.counts[w];
 		}
 		if (is && before < most) list[before] = score_alternative(key, (uint32_t) j);
 	}
@@ -107,9 +103,9 @@ __device__ __forceinline__ void score_select(const T * row, int first, int end, 
  * them (all of them where there are fewer than k). `groups`: the maxima that
  * the thread's batches left, SCORE_GROUP_SLOTS rows of blockDim.x. Returns n. */
 template <typename T>
-__device__ __forceinline__ int score_candidates(const T * row, const RowSlice & sl, int k, float row_max, const float * groups, uint16_t * reached, uint64_t * list, TopState & t) {
+__device__ __forceinline__ int score_candidates(const T * row, const RowSlice & sl, int k, float row_max, float met, float least, const float * groups, uint16_t * reached, uint64_t * list, TopState & t) {
 	constexpr int V = VecOf<T>::N;
-	const int tid = (int) threadIdx.x, nt = (int) blockDim.x;
+	const int tid = (int) threadIdx.x, nt = (int) blockDim.x, lane = tid & 63;
 	const int batches = (sl.last - sl.first + SCORE_BATCH * nt - 1) / (SCORE_BATCH * nt);
 	const int col0 = sl.first * V, col1 = sl.last * V + (sl.end - sl.tail);
 	const bool tail = sl.tail + tid < sl.end;
@@ -128,18 +124,14 @@ __device__ __forceinline__ int score_candidates(const T * row, const RowSlice & 
 		return (int) sl.columns(V);
 	}
 	float g[SCORE_GROUP_SLOTS];
-	float mine = -__builtin_inff();
 #pragma unroll
-	for (int i = 0; i < SCORE_GROUP_SLOTS; i++) {
-		g[i] = i < batches || i == 0 ? groups[i * nt + tid] : -__builtin_inff();
-		mine = fmaxf(mine, g[i]);
-	}
+	for (int i = 0; i < SCORE_GROUP_SLOTS; i++) g[i] = i < batches || i == 0 ? groups[i * nt + tid] : -__builtin_inff();
 	int turn = 0;
 	/* as many threads as have a column above -inf reach the least of their maxima */
-	const bool has = mine > -__builtin_inff();
-	float lo = -score_group_max(has ? -mine : -__builtin_inff(), t.cells);
+	float lo = least;
+	uint32_t reach = (uint32_t) met;
 	if (tid == 0) t.count = t.n_groups = 0u;
-	uint32_t reach = score_group_count((uint32_t) __popcll(__ballot(has)), t, turn);
+	lds_barrier();
 	if (reach >= (uint32_t) k) {
 		/* lo is reached by k groups or more, hi not known to be. Far from a row's
 		 * bulk the logarithm of how many reach a bound falls about evenly, so every
@@ -170,9 +162,15 @@ __device__ __forceinline__ int score_candidates(const T * row, const RowSlice & 
 	else lo = -3.402823466e38f;   /* few columns are above -inf: all of them */
 	/* the groups that reach it, and then a thread for each of their chunks */
 #pragma unroll
-	for (int i = 0; i < SCORE_GROUP_SLOTS; i++)
-		if (g[i] >= lo) reached[atomicAdd(&t.n_groups, 1u)] = (uint16_t) (i * nt + tid);
-	__syncthreads();
+	for (int i = 0; i < SCORE_GROUP_SLOTS; i++) {
+		const unsigned long long hit = __ballot(g[i] >= lo);
+		if (hit == 0ull) continue;
+		uint32_t at = 0u;
+		if (lane == 0) at = atomicAdd(&t.n_groups, (uint32_t) __popcll(hit));
+		at = __builtin_amdgcn_readfirstlane(at);
+		if (g[i] >= lo) reached[at + (uint32_t) __popcll(hit & ((1ull << lane) - 1ull))] = (uint16_t) (i * nt + tid);
+	}
+	lds_barrier();
 	const int items = (int) t.n_groups * SCORE_BATCH;
 #pragma unroll 1
 	for (int item = tid; item < items; item += nt) {
@@ -180,17 +178,21 @@ __device__ __forceinline__ int score_candidates(const T * row, const RowSlice & 
 #pragma unroll 1
 		for (int b = slot; b < batches || b == 0; b += SCORE_GROUP_SLOTS) {
 			const int c = sl.first + (b * SCORE_BATCH + item % SCORE_BATCH) * nt + owner;
-			if (c < sl.last) {
-				const R16 x = score_load(row, (uint64_t) c, 0u);
-				float f[V];
-				unpack16<T>(x, f);
+			if (c >= sl.last) continue;
+			const R16 x = score_load<T, true>(row, (uint64_t) c, 0u);
+			float f[V];
+			unpack16<T>(x, f);
+			uint32_t hits = 0u;
 #pragma unroll
-				for (int v = 0; v < V; v++)
-					if (f[v] >= lo) {
-						const uint32_t at = atomicAdd(&t.count, 1u);
-						if (at < SCORE_CANDIDATES) list[at] = score_alternative(score_key(f[v]), (uint32_t) (c * V + v));
-					}
-			}
+			for (int v = 0; v < V; v++) hits |= f[v] >= lo ? 1u << v : 0u;
+			if (hits == 0u) continue;
+			uint32_t at = atomicAdd(&t.count, (uint32_t) __popc(hits));
+#pragma unroll
+			for (int v = 0; v < V; v++)
+				if (hits >> v & 1u) {
+					if (at < SCORE_CANDIDATES) list[at] = score_alternative(score_key(f[v]), (uint32_t) (c * V + v));
+					at++;
+				}
 		}
 	}
 	if (tail) {
@@ -200,9 +202,9 @@ __device__ __forceinline__ int score_candidates(const T * row, const RowSlice & 
 			if (at < SCORE_CANDIDATES) list[at] = score_alternative(score_key(x), (uint32_t) (sl.tail + tid));
 		}
 	}
-	__syncthreads();
+	lds_barrier();
 	const int n = (int) t.count;
-	__syncthreads();
+	lds_barrier();
 	if (n > SCORE_CANDIDATES) {
 		score_select(row, col0, col1, k, list, t);
 		return k;
@@ -227,7 +229,7 @@ __device__ __forceinline__ void score_rank(const uint64_t * list, int n, const P
 	for (int i = (int) threadIdx.x >> 2; i < n; i += (int) (blockDim.x >> 2)) {
 		const uint64_t alt = list[i];
 		int r = 0;
-#pragma unroll 2
+#pragma unroll 4
 		for (int o = (int) threadIdx.x & 3; o < n; o += 4) r += list[o] > alt ? 1 : 0;
 		r += __builtin_amdgcn_update_dpp(0, r, DPP_QUAD_1032, 0xf, 0xf, false);
 		r += __builtin_amdgcn_update_dpp(0, r, DPP_QUAD_2301, 0xf, 0xf, false);
@@ -267,10 +269,10 @@ template <typename T, bool TOP>
 __device__ __forceinline__ void token_logprobs_run(const LogprobsArgs & a) {
 	constexpr int V = VecOf<T>::N;
 	__shared__ TopState t;
+	const Score_Plan plan = score_stream_plan(a.n_rows, a.n_cols, (int) sizeof(T), a.top_k);
 	extern __shared__ uint64_t list[];
 	float * groups = reinterpret_cast<float *>(list + SCORE_CANDIDATES);
 	uint16_t * reached = reinterpret_cast<uint16_t *>(groups + SCORE_GROUP_SLOTS * blockDim.x);
-	const Score_Plan plan = score_stream_plan(a.n_rows, a.n_cols, (int) sizeof(T));
 	const int tid = (int) threadIdx.x, nt = (int) blockDim.x;
 	const float s_log2e = a.s * SCORE_LOG2E;
 #pragma unroll 1
@@ -279,14 +281,14 @@ __device__ __forceinline__ void token_logprobs_run(const LogprobsArgs & a) {
 		const int slice = plan.slices == 1 ? 0 : (int) (w - r * plan.slices);
 		const T * row = static_cast<const T *>(a.logits) + (uint64_t) r * a.row_stride;
 		const RowSlice sl(a.n_cols, V, slice, plan.slices, plan.slice_chunks);
-		RowPart p = score_stream<T, true>(row, sl, s_log2e, TOP ? groups : nullptr);
-		p = score_group_join(p, s_log2e, t.cells);
+		float met, least;
+		const RowPart p = score_group_join<TOP>(score_stream<T, true, TOP>(row, sl, s_log2e, TOP ? groups : nullptr), s_log2e, t.cells, &met, &least);
 		const RowStats st(p.m, p.z, p.e);
 		if (plan.slices == 1) token_logprobs_row<T>(a, r, row, st);
 		else if (tid == 0) a.parts[w] = Score_Part{p.m, p.z, p.e, 0.0f};
 		if (TOP) {
 			const int k = a.top_k;
-			const int n = score_candidates(row, sl, k, p.m, groups, reached, list, t);
+			const int n = score_candidates(row, sl, k, p.m, met, least, groups, reached, list, t);
 			score_rank(list, n, [&](int rank, uint64_t alt) {
 				if (rank >= k) return;
 				if (plan.slices == 1) {
@@ -310,7 +312,7 @@ __device__ __forceinline__ void token_logprobs_join(const LogprobsArgs & a) {
 	extern __shared__ uint64_t list[];
 	__shared__ uint32_t count;
 	__shared__ unsigned long long all_reach, one_reaches;
-	const Score_Plan plan = score_stream_plan(a.n_rows, a.n_cols, (int) sizeof(T));
+	const Score_Plan plan = score_stream_plan(a.n_rows, a.n_cols, (int) sizeof(T), a.top_k);
 	const int tid = (int) threadIdx.x, nt = (int) blockDim.x, lane = tid & 63, k = a.top_k, slices = plan.slices;
 	const float s_log2e = a.s * SCORE_LOG2E;
 	for (long r = blockIdx.x; r < a.n_rows; r += gridDim.x) {
@@ -360,15 +362,15 @@ __device__ __forceinline__ void token_logprobs_join(const LogprobsArgs & a) {
 #define TOKEN_LOGPROBS_PACK                                                                                                      \
 	LogprobsArgs a = {n_rows, n_cols, row_stride, scale, tokens_per_row, top_k, logits, tokens, logprobs, entropy, lse, top_ids, \
 					  top_logprobs, nullptr, nullptr};                                                                           \
-	const Score_Plan plan = score_stream_plan(n_rows, n_cols, (int) sizeof(*logits));                                            \
+	const Score_Plan plan = score_stream_plan(n_rows, n_cols, (int) sizeof(*logits), top_k);                                            \
 	a.lists = static_cast<uint64_t *>(workspace);                                                                                \
 	a.parts = reinterpret_cast<Score_Part *>(a.lists + (uint64_t) n_rows * plan.slices * top_k);
 #define TOKEN_LOGPROBS_KERNEL(SUF, T)                                                                                            \
-	extern "C" __global__ void __launch_bounds__(64 * SCORE_STREAM_WAVES, 8) token_logprobs_##SUF##_kernel(TOKEN_LOGPROBS_ARGS(T)) { \
+	extern "C" __global__ void __launch_bounds__(64 * SCORE_MAX_WAVES, 8) token_logprobs_##SUF##_kernel(TOKEN_LOGPROBS_ARGS(T)) { \
 		TOKEN_LOGPROBS_PACK                                                                                                      \
 		token_logprobs_run<T, false>(a);                                                                                                \
 	}                                                                                                                            \
-	extern "C" __global__ void __launch_bounds__(64 * SCORE_STREAM_WAVES, 8) token_logprobs_##SUF##_kernel_top(TOKEN_LOGPROBS_ARGS(T)) { \
+	extern "C" __global__ void __launch_bounds__(64 * SCORE_STREAM_WAVES, 6) token_logprobs_##SUF##_kernel_top(TOKEN_LOGPROBS_ARGS(T)) { \
 		TOKEN_LOGPROBS_PACK                                                                                                      \
 		token_logprobs_run<T, true>(a);                                                                                          \
 	}                                                                                                                            \
