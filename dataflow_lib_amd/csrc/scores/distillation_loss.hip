@@ -89,7 +89,7 @@ __device__ __forceinline__ void distill_held(const DistillArgs & a) {
 	constexpr uint32_t E = (uint32_t) sizeof(T);
 	constexpr int B = CH < 4 ? CH : 4;   /* chunks that share a shift */
 	__shared__ DistillCells both[2];
-	extern __shared__ uint32_t entries[];   /* ids and values of two rows */
+	extern __shared__ uint4 entries[];   /* ids and values of two rows */
 	const int tid = (int) threadIdx.x, nt = NT ? NT : (int) blockDim.x, wave = tid >> 6, waves = nt >> 6, K = a.top_k;
 	const int chunks = a.n_cols / V, whole = chunks / nt;
 	const int have = whole + (tid < chunks - whole * nt ? 1 : 0);   /* this thread's chunks */
@@ -127,8 +127,8 @@ __device__ __forceinline__ void distill_held(const DistillArgs & a) {
 	int turn = 0;
 	for (; r < a.n_rows; turn ^= 1) {
 		DistillCells & cells = both[turn];
-		uint32_t * ids = entries + turn * 2 * K;
-		float * values = reinterpret_cast<float *>(ids + K);
+		uint32_t * ids = reinterpret_cast<uint32_t *>(entries) + turn * 2 * score_entries(K);
+		float * values = reinterpret_cast<float *>(ids + score_entries(K));
 		const long next = r + gridDim.x;
 		const float next_w = weight(next);
 		const uint32_t next_id = __builtin_amdgcn_raw_buffer_load_b32(ids_rsrc(next), entry_off, 0, 0);
@@ -173,7 +173,7 @@ __device__ __forceinline__ void distill_held(const DistillArgs & a) {
 			te.shift(wave_max(te.m), s_log2e);
 			te.z = wave_sum(te.z);
 		}
-		if (tid < K) {
+		if (tid < score_entries(K)) {
 			ids[tid] = is ? id : SCORE_NO_COLUMN;
 			values[tid] = v;
 		}
@@ -207,15 +207,25 @@ __device__ __forceinline__ void distill_held(const DistillArgs & a) {
 		if (wave * 64 < K) {
 			if (is && counts) {
 				const float d = a.s * (v - te.m);
-				float q = __builtin_amdgcn_exp2f(d * SCORE_LOG2E) / te.z;
+				const float q = __builtin_amdgcn_exp2f(d * SCORE_LOG2E) / te.z;
 				if (!(q == 0.0f)) l = q * ((d - logf(te.z)) - (st.none() ? -__builtin_inff() : st.log_p(xk, a.s)));
+				/* columns given twice: counted first, since there hardly are any */
+				int same = 0;
+#pragma unroll 4
+				for (int o = 0; o < score_entries(K) / 4; o++) {
+					const uint4 i4 = reinterpret_cast<const uint4 *>(ids)[o];
+					same += (i4.x == id) + (i4.y == id) + (i4.z == id) + (i4.w == id);
+				}
 				bool first = true;
-				float sum = 0.0f;
+				float sum = q;
+				if (same > 1) {
+					sum = 0.0f;
 #pragma unroll 1
-				for (int o = 0; o < K; o++) {
-					if (ids[o] != id) continue;
-					if (o < tid) first = false;
-					sum += __builtin_amdgcn_exp2f(a.s * (values[o] - te.m) * SCORE_LOG2E) / te.z;
+					for (int o = 0; o < K; o++) {
+						if (ids[o] != id) continue;
+						if (o < tid) first = false;
+						sum += __builtin_amdgcn_exp2f(a.s * (values[o] - te.m) * SCORE_LOG2E) / te.z;
+					}
 				}
 				if (first) fix_off = id * E;
 				fix = st.none() ? 0.0f : wt * (__builtin_amdgcn_exp2f((xk - st.max) * s_log2e) * st.inv_z - sum);
@@ -434,11 +444,11 @@ __device__ __forceinline__ void distillation_loss_mean(int n_rows, const float *
 		DISTILLATION_PACK \
 		distill_held<T, SCORE_HELD_MORE, 1024>(a); \
 	} \
-	extern "C" __global__ void __launch_bounds__(512, 2) distillation_loss_##SUF##_kernel_wide_rows(DISTILLATION_ARGS(T)) { \
+	extern "C" __global__ void __launch_bounds__(512, 4) distillation_loss_##SUF##_kernel_wide_rows(DISTILLATION_ARGS(T)) { \
 		DISTILLATION_PACK \
-		distill_held<T, SCORE_HELD_MORE, 512>(a); \
+		distill_held<T, SCORE_HELD_MORE, 0>(a); \
 	} \
-	extern "C" __global__ void __launch_bounds__(1024) distillation_loss_##SUF##_kernel_rows(DISTILLATION_ARGS(T)) { \
+	extern "C" __global__ void __launch_bounds__(1024, 8) distillation_loss_##SUF##_kernel_rows(DISTILLATION_ARGS(T)) { \
 		DISTILLATION_PACK \
 		distill_held<T, SCORE_HELD, 0>(a); \
 	} \

@@ -99,28 +99,31 @@ GEOM_FN unsigned long score_logprobs_workspace(int n_rows, int n_cols, int elem_
 
 /* distillation_loss with a gradient: rows that a workgroup holds in its
  * registers, with a thread per teacher entry. SCORE_HELD_ROWS: SCORE_HELD
- * chunks per thread and as many waves as that takes; SCORE_HELD_WIDE_ROWS and
- * SCORE_HELD_LONG_ROWS: SCORE_HELD_MORE chunks per thread, 8 and 16 waves. */
+ * chunks per thread in a wave or two (up to 16 where rows are few);
+ * SCORE_HELD_WIDE_ROWS and SCORE_HELD_LONG_ROWS: SCORE_HELD_MORE chunks per
+ * thread in up to 8 waves, and in 16. */
 #define SCORE_HELD 4
 #define SCORE_HELD_MORE 16
-#define SCORE_HELD_FEW 128
+#define SCORE_HELD_FEW 512
 #define SCORE_HELD_NONE 0
 #define SCORE_HELD_ROWS 1
 #define SCORE_HELD_WIDE_ROWS 2
 #define SCORE_HELD_LONG_ROWS 3
 GEOM_FN int score_held(int n_rows, int n_cols, int elem_bytes, int top_k) {
 	const long chunks = (long) n_cols * elem_bytes / 16;
-	if (chunks <= 16 * 64 * SCORE_HELD) return SCORE_HELD_ROWS;
-	if (n_rows < SCORE_HELD_FEW) return SCORE_HELD_NONE;
+	if (chunks <= (n_rows <= SCORE_HELD_FEW ? 16 : 2) * 64 * SCORE_HELD) return SCORE_HELD_ROWS;
+	if (n_rows < SCORE_HELD_FEW / 4) return SCORE_HELD_NONE;
 	if (chunks <= 8 * 64 * SCORE_HELD_MORE && top_k <= 8 * 64) return SCORE_HELD_WIDE_ROWS;
 	return chunks <= 16 * 64 * SCORE_HELD_MORE ? SCORE_HELD_LONG_ROWS : SCORE_HELD_NONE;
 }
 GEOM_FN int score_held_waves(int held, int n_cols, int elem_bytes, int top_k) {
-	if (held != SCORE_HELD_ROWS) return held == SCORE_HELD_WIDE_ROWS ? 8 : 16;
-	const int chunks = (int) ((long) n_cols * elem_bytes / 16);
-	const int waves = (chunks + 64 * SCORE_HELD - 1) / (64 * SCORE_HELD), entries = (top_k + 63) / 64;
+	if (held == SCORE_HELD_LONG_ROWS) return 16;
+	const int chunks = (int) ((long) n_cols * elem_bytes / 16), per_wave = 64 * (held == SCORE_HELD_ROWS ? SCORE_HELD : SCORE_HELD_MORE);
+	const int waves = (chunks + per_wave - 1) / per_wave, entries = (top_k + 63) / 64;
 	return waves > entries ? waves : entries > 0 ? entries : 1;
 }
+/* LDS: ids (padded to whole 16 bytes) and values of two rows' entries */
+GEOM_FN int score_entries(int top_k) { return (top_k + 3) & ~3; }
 
 /* a call may want the loss alone, whatever its sizes */
 GEOM_FN unsigned long score_distill_workspace(int n_rows, int n_cols, int elem_bytes, int top_k) {
@@ -133,10 +136,10 @@ GEOM_FN unsigned long score_distill_workspace(int n_rows, int n_cols, int elem_b
 /* token_logprobs: LDS of a workgroup with alternatives to find. Candidates,
  * group maxima (SCORE_GROUP_SLOTS per thread) and which of them reach a bound. */
 #define SCORE_GROUP_SLOTS 4
-#define SCORE_CANDIDATES 1024
+#define SCORE_CANDIDATES(waves) ((waves) <= 2 ? 512 : 1024)
 #define SCORE_FEW_COLUMNS 256   /* all of them are candidates */
 GEOM_FN unsigned score_top_lds(int waves) {
-	return (unsigned) (waves * 64 * SCORE_GROUP_SLOTS * 6 + SCORE_CANDIDATES * 8);
+	return (unsigned) (waves * 64 * SCORE_GROUP_SLOTS * 6 + SCORE_CANDIDATES(waves) * 8);
 }
 
 #endif

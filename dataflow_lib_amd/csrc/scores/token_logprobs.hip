@@ -99,6 +99,39 @@ __device__ __forceinline__ void score_select(const T * row, int first, int end, 
 	__syncthreads();
 }
 
+/* Where many more than k of a list's n numbers are left, those that reach a key
+ * that not many more than k reach, found by bisection and moved to the list's
+ * front. Returns how many. */
+__device__ __forceinline__ int score_thin(int n, int k, uint64_t * list, TopState & t, int & turn) {
+	const int tid = (int) threadIdx.x, nt = (int) blockDim.x, aim = k + (k >> 1) + 32;
+	if (n <= 2 * aim) return n;
+	uint32_t lo = 0u, hi = 0xffffffffu;   /* reached by k or more; not, or by none */
+	int reach = n;
+	if (tid == 0) t.count = 0u;
+#pragma unroll 1
+	while (reach > aim && hi - lo > 1u) {
+		const uint32_t mid = lo + ((hi - lo) >> 1);
+		uint32_t c = 0u;
+#pragma unroll 1
+		for (int i = tid; i < n + tid; i += nt) c += (uint32_t) __popcll(__ballot(i < n && (uint32_t) (list[i < n ? i : 0] >> 32) >= mid));
+		c = score_group_count(c, t, turn);
+		if (c < (uint32_t) k) hi = mid;
+		else {
+			lo = mid;
+			reach = (int) c;
+		}
+	}
+	/* what is kept of a step's numbers lies no further than the step's end */
+#pragma unroll 1
+	for (int i = tid; i < n + tid; i += nt) {
+		const uint64_t alt = i < n ? list[i] : 0u;
+		lds_barrier();
+		if (alt != 0u && (uint32_t) (alt >> 32) >= lo) list[atomicAdd(&t.count, 1u)] = alt;
+		lds_barrier();
+	}
+	return (int) t.count;
+}
+
 /* Candidates of a slice into list[0..n): the k largest of its columns among
  * them (all of them where there are fewer than k). `groups`: the maxima that
  * the thread's batches left, SCORE_GROUP_SLOTS rows of blockDim.x. Returns n. */
@@ -106,9 +139,11 @@ template <typename T>
 __device__ __forceinline__ int score_candidates(const T * row, const RowSlice & sl, int k, float row_max, float met, float least, const float * groups, uint16_t * reached, uint64_t * list, TopState & t) {
 	constexpr int V = VecOf<T>::N;
 	const int tid = (int) threadIdx.x, nt = (int) blockDim.x, lane = tid & 63;
+	const uint32_t most = SCORE_CANDIDATES(nt >> 6);
 	const int batches = (sl.last - sl.first + SCORE_BATCH * nt - 1) / (SCORE_BATCH * nt);
 	const int col0 = sl.first * V, col1 = sl.last * V + (sl.end - sl.tail);
 	const bool tail = sl.tail + tid < sl.end;
+	int turn = 0;
 	if (sl.columns(V) <= SCORE_FEW_COLUMNS) {
 		__syncthreads();
 #pragma unroll 1
@@ -121,12 +156,11 @@ __device__ __forceinline__ int score_candidates(const T * row, const RowSlice & 
 		}
 		if (tail) list[(sl.last - sl.first) * V + tid] = score_alternative(score_key(to_f(row[sl.tail + tid])), (uint32_t) (sl.tail + tid));
 		__syncthreads();
-		return (int) sl.columns(V);
+		return score_thin((int) sl.columns(V), k, list, t, turn);
 	}
 	float g[SCORE_GROUP_SLOTS];
 #pragma unroll
 	for (int i = 0; i < SCORE_GROUP_SLOTS; i++) g[i] = i < batches || i == 0 ? groups[i * nt + tid] : -__builtin_inff();
-	int turn = 0;
 	/* as many threads as have a column above -inf reach the least of their maxima */
 	float lo = least;
 	uint32_t reach = (uint32_t) met;
@@ -190,7 +224,7 @@ __device__ __forceinline__ int score_candidates(const T * row, const RowSlice & 
 #pragma unroll
 			for (int v = 0; v < V; v++)
 				if (hits >> v & 1u) {
-					if (at < SCORE_CANDIDATES) list[at] = score_alternative(score_key(f[v]), (uint32_t) (c * V + v));
+					if (at < most) list[at] = score_alternative(score_key(f[v]), (uint32_t) (c * V + v));
 					at++;
 				}
 		}
@@ -199,13 +233,13 @@ __device__ __forceinline__ int score_candidates(const T * row, const RowSlice & 
 		const float x = to_f(row[sl.tail + tid]);
 		if (x >= lo) {
 			const uint32_t at = atomicAdd(&t.count, 1u);
-			if (at < SCORE_CANDIDATES) list[at] = score_alternative(score_key(x), (uint32_t) (sl.tail + tid));
+			if (at < most) list[at] = score_alternative(score_key(x), (uint32_t) (sl.tail + tid));
 		}
 	}
 	lds_barrier();
 	const int n = (int) t.count;
 	lds_barrier();
-	if (n > SCORE_CANDIDATES) {
+	if (n > (int) most) {
 		score_select(row, col0, col1, k, list, t);
 		return k;
 	}
@@ -217,7 +251,7 @@ __device__ __forceinline__ int score_candidates(const T * row, const RowSlice & 
 		__syncthreads();
 		return (int) have;
 	}
-	return n;
+	return score_thin(n, k, list, t, turn);
 }
 
 /* The place of each of a list's n numbers among them, by counting the larger
@@ -271,7 +305,7 @@ __device__ __forceinline__ void token_logprobs_run(const LogprobsArgs & a) {
 	__shared__ TopState t;
 	const Score_Plan plan = score_stream_plan(a.n_rows, a.n_cols, (int) sizeof(T), a.top_k);
 	extern __shared__ uint64_t list[];
-	float * groups = reinterpret_cast<float *>(list + SCORE_CANDIDATES);
+	float * groups = reinterpret_cast<float *>(list + SCORE_CANDIDATES(plan.waves));
 	uint16_t * reached = reinterpret_cast<uint16_t *>(groups + SCORE_GROUP_SLOTS * blockDim.x);
 	const int tid = (int) threadIdx.x, nt = (int) blockDim.x;
 	const float s_log2e = a.s * SCORE_LOG2E;
