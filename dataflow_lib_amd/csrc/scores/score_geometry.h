@@ -136,10 +136,9 @@ GEOM_FN unsigned long score_distill_workspace(int n_rows, int n_cols, int elem_b
 /* token_logprobs: LDS of a workgroup with alternatives to find. Candidates,
  * group maxima (SCORE_GROUP_SLOTS per thread) and which of them reach a bound. */
 #define SCORE_GROUP_SLOTS 4
-#define SCORE_CANDIDATES(waves) ((waves) <= 2 ? 512 : 1024)
-#define SCORE_FEW_COLUMNS 256   /* all of them are candidates */
+#define SCORE_CANDIDATES 1024   /* all columns of a slice of so many */
 GEOM_FN unsigned score_top_lds(int waves) {
-	return (unsigned) (waves * 64 * SCORE_GROUP_SLOTS * 6 + SCORE_CANDIDATES(waves) * 8);
+	return (unsigned) (waves * 64 * SCORE_GROUP_SLOTS * 6 + SCORE_CANDIDATES * 8);
 }
 
 #endif

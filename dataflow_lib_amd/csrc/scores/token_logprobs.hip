@@ -99,34 +99,59 @@ __device__ __forceinline__ void score_select(const T * row, int first, int end, 
 	__syncthreads();
 }
 
-/* Where many more than k of a list's n numbers are left, those that reach a key
- * that not many more than k reach, found by bisection and moved to the list's
- * front. Returns how many. */
-__device__ __forceinline__ int score_thin(int n, int k, uint64_t * list, TopState & t, int & turn) {
-	const int tid = (int) threadIdx.x, nt = (int) blockDim.x, aim = k + (k >> 1) + 32;
-	if (n <= 2 * aim) return n;
-	uint32_t lo = 0u, hi = 0xffffffffu;   /* reached by k or more; not, or by none */
-	int reach = n;
-	if (tid == 0) t.count = 0u;
+/* A bound that `reach` numbers reach at `lo` (k or more of them) and none
+ * beyond `hi`, moved up until not many more than k reach it. Far from a row's
+ * bulk the logarithm of how many reach a bound falls about evenly, so every
+ * other step interpolates there; the others halve the interval. count(bound):
+ * how many reach it, over the workgroup. */
+template <typename Count>
+__device__ __forceinline__ float score_bound(float lo, float hi, uint32_t & reach, int k, const Count & count) {
+	const float aim = __builtin_amdgcn_logf(1.25f * (float) k + 2.0f);
+	float at_hi = 0.0f;
 #pragma unroll 1
-	while (reach > aim && hi - lo > 1u) {
-		const uint32_t mid = lo + ((hi - lo) >> 1);
-		uint32_t c = 0u;
-#pragma unroll 1
-		for (int i = tid; i < n + tid; i += nt) c += (uint32_t) __popcll(__ballot(i < n && (uint32_t) (list[i < n ? i : 0] >> 32) >= mid));
-		c = score_group_count(c, t, turn);
-		if (c < (uint32_t) k) hi = mid;
+	for (int step = 0; step < 24 && reach > (uint32_t) (k + (k >> 1) + 8); step++) {
+		const float at_lo = __builtin_amdgcn_logf((float) reach);
+		float part = 0.5f;
+		if (!(step & 1)) part = fminf(fmaxf((at_lo - aim) / (at_lo - at_hi), 0.02f), 0.98f);
+		const float mid = lo + part * (hi - lo);
+		if (!(mid > lo && mid <= hi)) break;
+		const uint32_t n = count(mid);
+		if (n < (uint32_t) k) {
+			hi = mid;
+			at_hi = n == 0u ? 0.0f : __builtin_amdgcn_logf((float) n);
+		}
 		else {
 			lo = mid;
-			reach = (int) c;
+			reach = n;
 		}
 	}
+	return lo;
+}
+
+/* Where many more than k of a list's n numbers are left (all of which reach lo,
+ * if any k do), those that reach a bound that not many more than k reach, moved
+ * to the list's front. Returns how many. */
+__device__ __forceinline__ int score_thin(int n, int k, float lo, float hi, uint64_t * list, TopState & t, int & turn) {
+	const int tid = (int) threadIdx.x, nt = (int) blockDim.x;
+	if (n <= 2 * k + 64) return n;
+	const uint32_t * keys = reinterpret_cast<const uint32_t *>(list) + 1;   /* the numbers' upper halves */
+	uint32_t reach = (uint32_t) n;
+	if (tid == 0) t.count = 0u;
+	lo = score_bound(lo, hi, reach, k, [&](float mid) {
+		const uint32_t key = score_key(mid);
+		uint32_t c = 0u;
+#pragma unroll 1
+		for (int i = tid; i < n + tid; i += nt) c += (uint32_t) __popcll(__ballot(i < n && keys[i < n ? 2 * i : 0] >= key));
+		return score_group_count(c, t, turn);
+	});
+	if (reach == (uint32_t) n) return n;
 	/* what is kept of a step's numbers lies no further than the step's end */
+	const uint32_t key = score_key(lo);
 #pragma unroll 1
 	for (int i = tid; i < n + tid; i += nt) {
 		const uint64_t alt = i < n ? list[i] : 0u;
 		lds_barrier();
-		if (alt != 0u && (uint32_t) (alt >> 32) >= lo) list[atomicAdd(&t.count, 1u)] = alt;
+		if ((uint32_t) (alt >> 32) >= key) list[atomicAdd(&t.count, 1u)] = alt;
 		lds_barrier();
 	}
 	return (int) t.count;
@@ -139,12 +164,11 @@ template <typename T>
 __device__ __forceinline__ int score_candidates(const T * row, const RowSlice & sl, int k, float row_max, float met, float least, const float * groups, uint16_t * reached, uint64_t * list, TopState & t) {
 	constexpr int V = VecOf<T>::N;
 	const int tid = (int) threadIdx.x, nt = (int) blockDim.x, lane = tid & 63;
-	const uint32_t most = SCORE_CANDIDATES(nt >> 6);
 	const int batches = (sl.last - sl.first + SCORE_BATCH * nt - 1) / (SCORE_BATCH * nt);
 	const int col0 = sl.first * V, col1 = sl.last * V + (sl.end - sl.tail);
 	const bool tail = sl.tail + tid < sl.end;
 	int turn = 0;
-	if (sl.columns(V) <= SCORE_FEW_COLUMNS) {
+	if (sl.columns(V) <= SCORE_CANDIDATES) {
 		__syncthreads();
 #pragma unroll 1
 		for (int c = sl.first + tid; c < sl.last; c += nt) {
@@ -156,7 +180,7 @@ __device__ __forceinline__ int score_candidates(const T * row, const RowSlice & 
 		}
 		if (tail) list[(sl.last - sl.first) * V + tid] = score_alternative(score_key(to_f(row[sl.tail + tid])), (uint32_t) (sl.tail + tid));
 		__syncthreads();
-		return score_thin((int) sl.columns(V), k, list, t, turn);
+		return met < (float) k ? (int) sl.columns(V) : score_thin((int) sl.columns(V), k, least, row_max, list, t, turn);
 	}
 	float g[SCORE_GROUP_SLOTS];
 #pragma unroll
@@ -167,31 +191,12 @@ __device__ __forceinline__ int score_candidates(const T * row, const RowSlice & 
 	if (tid == 0) t.count = t.n_groups = 0u;
 	lds_barrier();
 	if (reach >= (uint32_t) k) {
-		/* lo is reached by k groups or more, hi not known to be. Far from a row's
-		 * bulk the logarithm of how many reach a bound falls about evenly, so every
-		 * other bound is interpolated there; the others halve the interval. */
-		float hi = row_max, at_hi = 0.0f;
-		const float aim = __builtin_amdgcn_logf(1.25f * (float) k + 2.0f);
-#pragma unroll 1
-		for (int step = 0; step < 24 && reach > (uint32_t) (k + (k >> 1) + 8); step++) {
-			const float at_lo = __builtin_amdgcn_logf((float) reach);
-			float part = 0.5f;
-			if (!(step & 1)) part = fminf(fmaxf((at_lo - aim) / (at_lo - at_hi), 0.02f), 0.98f);
-			const float mid = lo + part * (hi - lo);
-			if (!(mid > lo && mid <= hi)) break;
+		lo = score_bound(lo, row_max, reach, k, [&](float mid) {
 			uint32_t n = 0;
 #pragma unroll
 			for (int i = 0; i < SCORE_GROUP_SLOTS; i++) n += (uint32_t) __popcll(__ballot(g[i] >= mid));
-			n = score_group_count(n, t, turn);
-			if (n < (uint32_t) k) {
-				hi = mid;
-				at_hi = n == 0u ? 0.0f : __builtin_amdgcn_logf((float) n);
-			}
-			else {
-				lo = mid;
-				reach = n;
-			}
-		}
+			return score_group_count(n, t, turn);
+		});
 	}
 	else lo = -3.402823466e38f;   /* few columns are above -inf: all of them */
 	/* the groups that reach it, and then a thread for each of their chunks */
@@ -224,7 +229,7 @@ __device__ __forceinline__ int score_candidates(const T * row, const RowSlice & 
 #pragma unroll
 			for (int v = 0; v < V; v++)
 				if (hits >> v & 1u) {
-					if (at < most) list[at] = score_alternative(score_key(f[v]), (uint32_t) (c * V + v));
+					if (at < SCORE_CANDIDATES) list[at] = score_alternative(score_key(f[v]), (uint32_t) (c * V + v));
 					at++;
 				}
 		}
@@ -233,13 +238,13 @@ __device__ __forceinline__ int score_candidates(const T * row, const RowSlice & 
 		const float x = to_f(row[sl.tail + tid]);
 		if (x >= lo) {
 			const uint32_t at = atomicAdd(&t.count, 1u);
-			if (at < most) list[at] = score_alternative(score_key(x), (uint32_t) (sl.tail + tid));
+			if (at < SCORE_CANDIDATES) list[at] = score_alternative(score_key(x), (uint32_t) (sl.tail + tid));
 		}
 	}
 	lds_barrier();
 	const int n = (int) t.count;
 	lds_barrier();
-	if (n > (int) most) {
+	if (n > SCORE_CANDIDATES) {
 		score_select(row, col0, col1, k, list, t);
 		return k;
 	}
@@ -251,7 +256,7 @@ __device__ __forceinline__ int score_candidates(const T * row, const RowSlice & 
 		__syncthreads();
 		return (int) have;
 	}
-	return score_thin(n, k, list, t, turn);
+	return score_thin(n, k, lo, row_max, list, t, turn);
 }
 
 /* The place of each of a list's n numbers among them, by counting the larger
@@ -305,7 +310,7 @@ __device__ __forceinline__ void token_logprobs_run(const LogprobsArgs & a) {
 	__shared__ TopState t;
 	const Score_Plan plan = score_stream_plan(a.n_rows, a.n_cols, (int) sizeof(T), a.top_k);
 	extern __shared__ uint64_t list[];
-	float * groups = reinterpret_cast<float *>(list + SCORE_CANDIDATES(plan.waves));
+	float * groups = reinterpret_cast<float *>(list + SCORE_CANDIDATES);
 	uint16_t * reached = reinterpret_cast<uint16_t *>(groups + SCORE_GROUP_SLOTS * blockDim.x);
 	const int tid = (int) threadIdx.x, nt = (int) blockDim.x;
 	const float s_log2e = a.s * SCORE_LOG2E;

@@ -107,8 +107,13 @@ def close(o, v, tol, what):
 
 def rounded_once(o, dt, v, slack, what):
     """outputs of type dt: the rounding (half a step) of a value within `slack`
-    of v; fp32's subnormal range may flush to zero"""
+    of v; fp32's subnormal range may flush to zero. fp16 ends at 65504, so what
+    lies half a step (16) beyond rounds to infinity, and only that."""
     of, v = to_f64(o, dt), np.asarray(v, np.float64)
+    if dt == FP16:
+        beyond = np.isinf(of)
+        assert (np.sign(of) * v + slack)[beyond].min(initial=np.inf) >= 65520.0 and (np.abs(v) - slack)[~beyond].max(initial=0.0) < 65520.0 or np.isnan(v).any(), what
+        of = np.where(beyond & np.isfinite(v), v, of)
     nan = np.isnan(v)
     assert np.array_equal(np.isnan(of), nan), what + ": NaN in other places"
     off = np.abs(of - v) - (0.5 * ulp(np.abs(v) + slack, dt) + slack + 2.0 * FTZ_LIMIT)

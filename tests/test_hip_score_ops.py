@@ -58,7 +58,8 @@ def check_logprobs(dt, x, n_cols, scale, tokens, top_k, got, what=""):
 SHAPES = [(1, 1, 0, 0, 1, 1), (3, 2, 1, 1, 2, 2), (5, 7, 0, 0, 1, 7), (7, 64, 0, 0, 3, 8), (9, 65, 3, 0, 2, 65), (33, 1000, 0, 0, 1, 20), (300, 255, 1, 3, 1, 5),
           (17, 2049, 0, 5, 4, 64), (70, 8192, 0, 0, 1, 1), (5, 16385, 15, 0, 1, 128), (64, 32000, 64, 0, 4, 10), (4, 50257, 0, 0, 1, 256), (600, 4099, 0, 0, 1, 40),
           (2, 128256, 0, 0, 1, 20), (1, 151937, 0, 1, 1, 100), (3, 300001, 7, 0, 5, 256), (130, 65537, 0, 0, 1, 0), (257, 40000, 0, 0, 0, 3), (12, 131072, 0, 8, 1, 33),
-          (2500, 300, 20, 0, 1, 7), (1, 1 << 21, 0, 0, 2, 50)]
+          (2500, 300, 20, 0, 1, 7), (1, 1 << 21, 0, 0, 2, 50), (1, 1 << 21, 1, 0, 1, 256), (2, 128257, 0, 0, 3, 0), (60, 1000, 0, 0, 1, 256),
+          (90, 513, 0, 1, 1, 30)]
 
 
 @pytest.mark.parametrize("dt", DTS, ids=dt_id)
@@ -466,6 +467,121 @@ def test_captured_and_replayed(hdl, shape):
             for a, b, n in zip(replayed[0], eager[0], sizes):
                 assert np.array_equal(d.get(a, (n,), np.uint8), d.get(b, (n,), np.uint8)), "replay %d" % i
         graph.destroy()
+
+
+# each of the kernels that hold rows, with several rows to a workgroup: a wave,
+# a few waves, 16 waves
+WALKED = [(9001, 301, 0, 7), (800, 40001, 3, 30), (600, 66000, 0, 64)]
+
+
+@pytest.mark.parametrize("dt", [BF16, FP16], ids=dt_id)
+@pytest.mark.parametrize("shape", WALKED, ids=lambda s: "%dx%d+%d_k%d" % s)
+def test_distillation_walks_rows(hdl, dt, shape):
+    """workgroups that take several rows: the next row's logits, teacher and
+    weight arrive while a row leaves; rows without weight and rows without an
+    entry lie between the others"""
+    n_rows, n_cols, pad, k = shape
+    x = logits(n_cols, (n_rows, n_cols), n_cols + pad, dt)
+    ids, v = teacher_for(n_rows, n_rows, n_cols, k)
+    wt = np.where(rng(3).random(n_rows) < 0.2, 0.0, rng(4).uniform(0.1, 2.0, n_rows)).astype(np.float32)
+    ids[5::97] = NO_TOKEN
+    check_distill(dt, x, n_cols, 0.5, ids, v, wt, run_distill(hdl, dt, x, n_cols, 0.5, ids, v, wt))
+
+
+def test_more_rows_than_workgroups(hdl):
+    """1.2 million short rows"""
+    n_rows, n_cols, k, m = 1200003, 8, 2, 1
+    x = np.tile(logits(110, (3001, n_cols), n_cols, FP32), (400, 1))[:n_rows]
+    x = np.ascontiguousarray(np.resize(x, (n_rows, n_cols)))
+    tok = np.resize(tokens_for(111, 3001, n_cols, m), (n_rows, m))
+    got = run_logprobs(hdl, FP32, x, n_cols, 1.0, tok, k)
+    check_logprobs(FP32, x, n_cols, 1.0, tok, k, got)
+    g, he = normal_f32(112, (n_rows, m)), normal_f32(113, (n_rows,))
+    out = run_grad(hdl, FP32, x, n_cols, 1.0, tok, got["lse"], got["entropy"], g, he)
+    rounded_once(out, FP32, want_grad(FP32, x, n_cols, 1.0, tok, got["lse"], got["entropy"], g, he),
+                 grad_slack(FP32, x, n_cols, 1.0, tok, got["lse"], got["entropy"], g, he), "dlogits")
+    ids, v = (np.resize(a, (n_rows, 3)) for a in teacher_for(114, 3001, n_cols, 3))
+    check_distill(FP32, x, n_cols, 1.0, ids, v, None, run_distill(hdl, FP32, x, n_cols, 1.0, ids, v, None))
+
+
+@pytest.mark.parametrize("dt", DTS, ids=dt_id)
+@pytest.mark.parametrize("scale", [1e-6, 1e6])
+def test_scales_at_the_limits(hdl, dt, scale):
+    """nearly uniform rows, and rows whose largest logit takes everything"""
+    n_rows, n_cols, k = 6, 5000, 20
+    x = logits(120, (n_rows, n_cols), n_cols, dt)
+    tok = tokens_for(121, n_rows, n_cols, 2)
+    s32 = float(np.float32(scale))
+    got = run_logprobs(hdl, dt, x, n_cols, scale, tok, k)
+    w = want_logprobs(dt, x, n_cols, scale, tok, k)
+    assert np.array_equal(got["top_ids"], w["top_ids"])
+    close(got["logprobs"], w["logprobs"], logprob_tol(n_cols, w["logprobs"]), "logprobs")
+    close(got["entropy"], w["entropy"], entropy_tol(n_cols), "entropy")
+    ids, v = teacher_for(122, n_rows, n_cols, 5)
+    loss, mean, dx = run_distill(hdl, dt, x, n_cols, scale, ids, v, None)
+    l, m, d = want_distill(dt, x, n_cols, scale, ids, v, None)
+    # differences of logarithms reach s times the logits' spread, about 40
+    close(loss, l, distill_loss_tol(n_cols, scale, 5) + np.abs(l) * 16 * U32 + 64.0 * max(s32, 1.0) / s32 ** 2 * 64.0 * U32, "loss")
+    rounded_once(dx, dt, d, distill_slack(dt, x, n_cols, scale, ids, None), "dlogits")
+
+
+def test_a_row_of_more_than_4_gib(hdl):
+    """one row of 2^31 - 2^24 bf16 logits, a block of 2^24 again and again: its
+    log-sum-exp is the block's and log(127), the largest logits' first
+    occurrences come first, and the gradient is the same in every block"""
+    block, times, k = 1 << 24, 127, 5
+    n_cols = block * times
+    x = logits(130, (1, block), block, BF16)
+    w = want_logprobs(BF16, x, block, 1.0, np.zeros((1, 1), np.uint32), k)
+    order = w["top_ids"][0].astype(np.int64)
+    tok = np.array([[n_cols - 1, 3]], np.uint32)
+    lse = w["lse"] + np.log(times)
+    ids, v = np.array([[n_cols - 2, 7]], np.uint32), np.array([[1.0, 0.5]], np.float32)
+    xf = to_f64(x, BF16)[0]
+    with Dev(hdl) as d:
+        p = d.empty(2 * n_cols)
+        ptok, plp, pe, pl, pi, pv = d.put(tok), d.empty(8), d.empty(4), d.empty(4), d.empty(4 * k), d.empty(4 * k)
+        pids, pvals, ploss, pg, ph = d.put(ids), d.put(v), d.empty(4), d.put(np.array([[0.5, -2.0]], np.float32)), d.put(np.array([0.25], np.float32))
+        s1, s2 = space(d, api.token_logprobs_workspace(BF16, 1, n_cols, k)), space(d, api.distillation_loss_workspace(BF16, 1, n_cols, 2))
+
+        def fill():
+            hdl.to_device(x, p)
+            for i in range(1, times):
+                assert hdl.copy(p + 2 * block * i, p, 2 * block) == 0
+
+        def blocks():
+            hdl.sync()
+            return [hdl.to_host(p + 2 * block * i, (block,), np.uint16) for i in (0, 63, times - 1)]
+
+        fill()
+        assert api.submit_token_logprobs(hdl, 0, BF16, 1, n_cols, n_cols, 1.0, 2, k, p, ptok, plp, pe, pl, pi, pv, *s1) == 0
+        # per-thread sums of 2^19 and more terms: the depth of the sums is that of the longest thread
+        slack = 2.0 ** 20 * U32
+        got_l, got_e = d.get(pl, (1,), np.float32), d.get(pe, (1,), np.float32)
+        close(got_l, lse, slack, "lse")
+        close(got_e, w["entropy"] + np.log(times), 20.0 * slack, "entropy")
+        close(d.get(plp, (2,), np.float32), xf[[block - 1, 3]] - lse, slack, "logprobs")
+        top = np.concatenate([np.arange(times) * block + order[0]])[:k]
+        assert np.array_equal(d.get(pi, (k,), np.uint32), top.astype(np.uint32))
+        assert api.submit_token_logprobs_bwd(hdl, 0, BF16, 1, n_cols, n_cols, n_cols, 1.0, 2, p, ptok, pl, pe, pg, ph, p) == 0
+        lp = xf - float(got_l[0])
+        dx = -np.exp(lp) * (-1.5 + 0.25 * (lp + float(got_e[0])))
+        first, mid, last = blocks()
+        want = dx.copy()
+        rounded_once(mid, BF16, want, np.exp(lp) * 64.0 * (4 * np.abs(lp) + 16) * U32, "the middle block")
+        at = np.array([3])
+        assert np.array_equal(np.delete(first, at), np.delete(mid, at)) and np.array_equal(last[:-1], mid[:-1])
+        assert abs(to_f64(last, BF16)[-1] - (dx[-1] + 0.5)) <= 2.0 ** -9 and abs(to_f64(first, BF16)[3] - (dx[3] - 2.0)) <= 2.0 ** -8
+        fill()
+        assert api.submit_distillation_loss(hdl, 0, BF16, 1, n_cols, n_cols, n_cols, 1.0, 2, p, pids, pvals, None, ploss, None, p, *s2) == 0
+        q = np.exp(v[0].astype(np.float64) - 1.0)
+        q /= q.sum()
+        close(d.get(ploss, (1,), np.float32), [(q * (np.log(q) - (xf[[block - 2, 7]] - lse[0]))).sum()], 2.0 * slack, "loss")
+        first, mid, last = blocks()
+        pr = np.exp(xf - lse[0])
+        rounded_once(mid, BF16, pr, pr * 2.0 * slack, "the middle block")
+        assert np.array_equal(np.delete(first, 7), np.delete(mid, 7)) and np.array_equal(np.delete(last, block - 2), np.delete(mid, block - 2))
+        assert abs(to_f64(last, BF16)[block - 2] - (pr[block - 2] - q[0])) <= 2.0 ** -9 and abs(to_f64(first, BF16)[7] - (pr[7] - q[1])) <= 2.0 ** -9
 
 
 def test_rows_beyond_4_gib(hdl):
