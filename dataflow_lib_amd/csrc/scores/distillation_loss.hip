@@ -91,15 +91,20 @@ __device__ __forceinline__ void distill_held(const DistillArgs & a) {
 	__shared__ DistillCells both[2];
 	extern __shared__ uint4 entries[];   /* ids and values of two rows */
 	const int tid = (int) threadIdx.x, nt = NT ? NT : (int) blockDim.x, wave = tid >> 6, waves = nt >> 6, K = a.top_k;
-	const int chunks = a.n_cols / V, whole = chunks / nt;
-	const int have = whole + (tid < chunks - whole * nt ? 1 : 0);   /* this thread's chunks */
 	const float s_log2e = a.s * SCORE_LOG2E, temperature = 1.0f / a.s;
 	const uint32_t voff = (uint32_t) tid * 16u;
-	const uint32_t tail_off = chunks * V + tid < a.n_cols ? (uint32_t) (chunks * V + tid) * E : SCORE_NOWHERE;
-	const uint32_t row_bytes = (uint32_t) a.n_cols * E, chunk_bytes = (uint32_t) chunks * 16u;
+	const uint32_t row_bytes = (uint32_t) a.n_cols * E;
 	const uint32_t entry_off = tid < K ? (uint32_t) tid * 4u : SCORE_NOWHERE;
 
 	const auto row_ptr = [&](long r) { return static_cast<const T *>(a.logits) + (uint64_t) r * a.row_stride; };
+	const auto out_ptr = [&](long r) { return static_cast<T *>(a.dlogits) + (uint64_t) r * a.grad_stride; };
+	/* chunks lie as the gradient's do */
+	const auto head_of = [&](long r) { return score_head(out_ptr(r), a.n_cols); };
+	/* this thread's element of a row's head or tail */
+	const auto single_off = [&](int head) {
+		const int tail = head + (a.n_cols - head) / V * V, e = tid < head ? tid : tail + tid - head;
+		return e < a.n_cols ? (uint32_t) e * E : SCORE_NOWHERE;
+	};
 	const auto weight = [&](long r) { return r >= a.n_rows ? 0.0f : a.weights ? load_scalar(a.weights + r) : 1.0f; };
 	const auto ids_rsrc = [&](long r) { return make_rsrc(a.ids + (uint64_t) r * K, r < a.n_rows ? (uint32_t) K * 4u : 0u); };
 	const auto values_rsrc = [&](long r) { return make_rsrc(a.values + (uint64_t) r * K, r < a.n_rows ? (uint32_t) K * 4u : 0u); };
@@ -107,6 +112,8 @@ __device__ __forceinline__ void distill_held(const DistillArgs & a) {
 
 	long r = blockIdx.x;
 	float w = weight(r);
+	int head = head_of(r), chunks = (a.n_cols - head) / V;
+	uint32_t single = single_off(head);
 	R16 x[CH];
 	uint32_t id;
 	float v, xk, xt;
@@ -114,11 +121,11 @@ __device__ __forceinline__ void distill_held(const DistillArgs & a) {
 		id = __builtin_amdgcn_raw_buffer_load_b32(ids_rsrc(r), entry_off, 0, 0);
 		v = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(values_rsrc(r), entry_off, 0, 0));
 		const bool there = w != 0.0f;
-		const __amdgpu_buffer_rsrc_t rs = make_rsrc(row_ptr(r), there ? chunk_bytes : 0u);
+		const __amdgpu_buffer_rsrc_t rs = make_rsrc(row_ptr(r) + head, there ? (uint32_t) chunks * 16u : 0u);
 #pragma unroll
 		for (int j = 0; j < CH; j++) x[j] = buf_load16_nt(rs, voff, (uint32_t) (j * nt) * 16u);
 		const __amdgpu_buffer_rsrc_t re = make_rsrc(row_ptr(r), there ? row_bytes : 0u);
-		xt = buf_load_elem<T>(re, tail_off);
+		xt = buf_load_elem<T>(re, single);
 		xk = buf_load_elem<T>(re, pick_off(id));
 	}
 	long before = -1;                        /* the row whose teacher columns and loss are still to be stored */
@@ -136,15 +143,15 @@ __device__ __forceinline__ void distill_held(const DistillArgs & a) {
 
 		/* statistics */
 		RowPart p;
-		const float xtail = tail_off != SCORE_NOWHERE ? xt : -__builtin_inff();
-		p.m = fmaxf(xtail, -__builtin_inff());
-		p.z = __builtin_amdgcn_exp2f((xtail - (p.m == -__builtin_inff() ? 0.0f : p.m)) * s_log2e);
+		const float xs = single != SCORE_NOWHERE ? xt : -__builtin_inff();
+		p.m = fmaxf(xs, -__builtin_inff());
+		p.z = __builtin_amdgcn_exp2f((xs - (p.m == -__builtin_inff() ? 0.0f : p.m)) * s_log2e);
 #pragma unroll
 		for (int j0 = 0; j0 < CH; j0 += B) {
 			float m = -__builtin_inff();
 #pragma unroll
 			for (int j = j0; j < j0 + B; j++) {
-				if (j >= have) continue;
+				if (j * nt + tid >= chunks) continue;
 				float f[V];
 				unpack16<T>(x[j], f);
 #pragma unroll
@@ -155,7 +162,7 @@ __device__ __forceinline__ void distill_held(const DistillArgs & a) {
 			float z[2] = {0.0f, 0.0f};
 #pragma unroll
 			for (int j = j0; j < j0 + B; j++) {
-				if (j >= have) continue;
+				if (j * nt + tid >= chunks) continue;
 				__builtin_amdgcn_sched_barrier(0);
 				reg_barrier(x[j]);
 				float f[V];
@@ -186,7 +193,7 @@ __device__ __forceinline__ void distill_held(const DistillArgs & a) {
 		__builtin_amdgcn_s_waitcnt(0x0F70);   /* vmcnt(0): all of it is behind the last chunk, which is here */
 		lds_barrier();
 		if (before >= 0) {
-			if (a.dlogits) buf_store_elem<T>(make_rsrc(static_cast<T *>(a.dlogits) + (uint64_t) before * a.grad_stride, row_bytes), fix_off, fix);
+			buf_store_elem<T>(make_rsrc(out_ptr(before), row_bytes), fix_off, fix);
 			if (tid == 0) {
 				float l = 0.0f;
 				for (int i = 0; i * 64 < K; i++) l += both[turn ^ 1].loss[i];
@@ -237,10 +244,11 @@ __device__ __forceinline__ void distill_held(const DistillArgs & a) {
 		/* the gradient, and the next row */
 		const bool zero = !counts || st.none();
 		const float scale = zero ? 0.0f : wt * st.inv_z, ref = st.max;
-		const __amdgpu_buffer_rsrc_t rs = make_rsrc(row_ptr(next), next_w != 0.0f ? chunk_bytes : 0u);
+		const int next_head = next < a.n_rows ? head_of(next) : 0, next_chunks = (a.n_cols - next_head) / V;
+		const __amdgpu_buffer_rsrc_t rs = make_rsrc(row_ptr(next) + next_head, next_w != 0.0f ? (uint32_t) next_chunks * 16u : 0u);
 		const __amdgpu_buffer_rsrc_t re = make_rsrc(row_ptr(next), next_w != 0.0f ? row_bytes : 0u);
-		T * out = static_cast<T *>(a.dlogits) + (uint64_t) r * a.grad_stride;
-		const __amdgpu_buffer_rsrc_t ro = make_rsrc(out, chunk_bytes);
+		T * out = out_ptr(r);
+		const __amdgpu_buffer_rsrc_t ro = make_rsrc(out + head, (uint32_t) chunks * 16u);
 		const auto grad = [&](float f) { return zero ? 0.0f : scale * __builtin_amdgcn_exp2f((f - ref) * s_log2e); };
 #pragma unroll
 		for (int j = 0; j < CH; j++) {
@@ -253,8 +261,11 @@ __device__ __forceinline__ void distill_held(const DistillArgs & a) {
 			buf_store16_nt(ro, voff, (uint32_t) (j * nt) * 16u, pack16<T>(f));
 			x[j] = buf_load16_nt(rs, voff, (uint32_t) (j * nt) * 16u);
 		}
-		buf_store_elem<T>(make_rsrc(out, row_bytes), tail_off, grad(xtail));
-		xt = buf_load_elem<T>(re, tail_off);
+		buf_store_elem<T>(make_rsrc(out, row_bytes), single, grad(xs));
+		head = next_head;
+		chunks = next_chunks;
+		single = single_off(head);
+		xt = buf_load_elem<T>(re, single);
 		xk = buf_load_elem<T>(re, pick_off(next_id));
 		before = r;
 		r = next;
@@ -265,7 +276,7 @@ __device__ __forceinline__ void distill_held(const DistillArgs & a) {
 	__builtin_amdgcn_s_waitcnt(0x0F70);
 	lds_barrier();
 	if (before >= 0) {
-		buf_store_elem<T>(make_rsrc(static_cast<T *>(a.dlogits) + (uint64_t) before * a.grad_stride, row_bytes), fix_off, fix);
+		buf_store_elem<T>(make_rsrc(out_ptr(before), row_bytes), fix_off, fix);
 		if (tid == 0) {
 			float l = 0.0f;
 			for (int i = 0; i * 64 < K; i++) l += both[turn ^ 1].loss[i];
@@ -340,7 +351,7 @@ __device__ __forceinline__ void distill_parts(const DistillArgs & a) {
 			if (alone && threadIdx.x == 0) a.loss[r] = 0.0f;
 			continue;
 		}
-		const RowSlice sl(a.n_cols, VecOf<T>::N, slice, plan.slices, plan.slice_chunks);
+		const RowSlice sl(a.n_cols, VecOf<T>::N, score_head(row, a.n_cols), slice, plan.slices, plan.slice_chunks);
 		const RowPart p = score_group_join<false>(score_stream<T, false, false>(row, sl, s_log2e, nullptr), s_log2e, cells);
 		if (alone) {
 			distill_teacher(a, r, RowStats(p.m, p.z, 0.0f), true, te, cells, [&](int, uint32_t id) { return to_f(row[id]); });
@@ -370,7 +381,7 @@ __device__ __forceinline__ void distill_out(const DistillArgs & a) {
 		const T * row = static_cast<const T *>(a.logits) + (uint64_t) r * a.row_stride;
 		T * out = a.dlogits ? static_cast<T *>(a.dlogits) + (uint64_t) r * a.grad_stride : nullptr;
 		if (!out && slice > 0) continue;
-		const RowSlice sl(a.n_cols, VecOf<T>::N, slice, plan.slices, plan.slice_chunks);
+		const RowSlice sl(a.n_cols, VecOf<T>::N, out ? score_head(out, a.n_cols) : 0, slice, plan.slices, plan.slice_chunks);
 		const float w = a.weights ? a.weights[r] : 1.0f;
 		if (w == 0.0f) {
 			if (slice == 0 && threadIdx.x == 0) a.loss[r] = 0.0f;

@@ -165,22 +165,22 @@ __device__ __forceinline__ int score_candidates(const T * row, const RowSlice & 
 	constexpr int V = VecOf<T>::N;
 	const int tid = (int) threadIdx.x, nt = (int) blockDim.x, lane = tid & 63;
 	const int batches = (sl.last - sl.first + SCORE_BATCH * nt - 1) / (SCORE_BATCH * nt);
-	const int col0 = sl.first * V, col1 = sl.last * V + (sl.end - sl.tail);
-	const bool tail = sl.tail + tid < sl.end;
+	const int col0 = sl.begin(V), col1 = sl.behind(V), single = sl.single();
+	const T * chunks = row + sl.head;
 	int turn = 0;
-	if (sl.columns(V) <= SCORE_CANDIDATES) {
+	if (col1 - col0 <= SCORE_CANDIDATES) {
 		__syncthreads();
 #pragma unroll 1
 		for (int c = sl.first + tid; c < sl.last; c += nt) {
-			R16 x = score_load(row, (uint64_t) c, 0u);
+			R16 x = score_load(chunks, (uint64_t) c, 0u);
 			float f[V];
 			unpack16<T>(x, f);
 #pragma unroll
-			for (int i = 0; i < V; i++) list[(c - sl.first) * V + i] = score_alternative(score_key(f[i]), (uint32_t) (c * V + i));
+			for (int i = 0; i < V; i++) list[sl.head + c * V + i - col0] = score_alternative(score_key(f[i]), (uint32_t) (sl.head + c * V + i));
 		}
-		if (tail) list[(sl.last - sl.first) * V + tid] = score_alternative(score_key(to_f(row[sl.tail + tid])), (uint32_t) (sl.tail + tid));
+		if (single >= 0) list[single - col0] = score_alternative(score_key(to_f(row[single])), (uint32_t) single);
 		__syncthreads();
-		return met < (float) k ? (int) sl.columns(V) : score_thin((int) sl.columns(V), k, least, row_max, list, t, turn);
+		return met < (float) k ? col1 - col0 : score_thin(col1 - col0, k, least, row_max, list, t, turn);
 	}
 	float g[SCORE_GROUP_SLOTS];
 #pragma unroll
@@ -218,7 +218,7 @@ __device__ __forceinline__ int score_candidates(const T * row, const RowSlice & 
 		for (int b = slot; b < batches || b == 0; b += SCORE_GROUP_SLOTS) {
 			const int c = sl.first + (b * SCORE_BATCH + item % SCORE_BATCH) * nt + owner;
 			if (c >= sl.last) continue;
-			const R16 x = score_load<T, true>(row, (uint64_t) c, 0u);
+			const R16 x = score_load<T, true>(chunks, (uint64_t) c, 0u);
 			float f[V];
 			unpack16<T>(x, f);
 			uint32_t hits = 0u;
@@ -229,16 +229,16 @@ __device__ __forceinline__ int score_candidates(const T * row, const RowSlice & 
 #pragma unroll
 			for (int v = 0; v < V; v++)
 				if (hits >> v & 1u) {
-					if (at < SCORE_CANDIDATES) list[at] = score_alternative(score_key(f[v]), (uint32_t) (c * V + v));
+					if (at < SCORE_CANDIDATES) list[at] = score_alternative(score_key(f[v]), (uint32_t) (sl.head + c * V + v));
 					at++;
 				}
 		}
 	}
-	if (tail) {
-		const float x = to_f(row[sl.tail + tid]);
+	if (single >= 0) {
+		const float x = to_f(row[single]);
 		if (x >= lo) {
 			const uint32_t at = atomicAdd(&t.count, 1u);
-			if (at < SCORE_CANDIDATES) list[at] = score_alternative(score_key(x), (uint32_t) (sl.tail + tid));
+			if (at < SCORE_CANDIDATES) list[at] = score_alternative(score_key(x), (uint32_t) single);
 		}
 	}
 	lds_barrier();
@@ -319,7 +319,7 @@ __device__ __forceinline__ void token_logprobs_run(const LogprobsArgs & a) {
 		const long r = plan.slices == 1 ? w : w / plan.slices;
 		const int slice = plan.slices == 1 ? 0 : (int) (w - r * plan.slices);
 		const T * row = static_cast<const T *>(a.logits) + (uint64_t) r * a.row_stride;
-		const RowSlice sl(a.n_cols, V, slice, plan.slices, plan.slice_chunks);
+		const RowSlice sl(a.n_cols, V, score_head(row, a.n_cols), slice, plan.slices, plan.slice_chunks);
 		float met, least;
 		const RowPart p = score_group_join<TOP>(score_stream<T, true, TOP>(row, sl, s_log2e, TOP ? groups : nullptr), s_log2e, t.cells, &met, &least);
 		const RowStats st(p.m, p.z, p.e);

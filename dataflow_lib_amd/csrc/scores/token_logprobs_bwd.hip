@@ -66,9 +66,9 @@ __device__ __forceinline__ void token_logprobs_bwd_run(int n_rows, int n_cols, u
 	for (long w = blockIdx.x; w < (long) n_rows * plan.slices; w += gridDim.x) {
 		const long r = plan.slices == 1 ? w : w / plan.slices;
 		const int slice = plan.slices == 1 ? 0 : (int) (w - r * plan.slices);
-		const RowSlice sl(n_cols, V, slice, plan.slices, plan.slice_chunks);
 		const T * row = logits + (uint64_t) r * row_stride;
 		T * out = dlogits + (uint64_t) r * grad_stride;
+		const RowSlice sl(n_cols, V, score_head(out, n_cols), slice, plan.slices, plan.slice_chunks);   /* stores aligned */
 		__syncthreads();
 		float down = 0.0f, any = 0.0f;
 		for (int m = (int) threadIdx.x; m < tokens_per_row; m += (int) blockDim.x) {
