@@ -191,7 +191,8 @@ int distillation_loss_set_launch_config(Hip_Launch_Config * hip_launch_config, D
 	if (held) {
 		const int waves = score_held_waves(held, n_cols, (int) elem, top_k);
 		const unsigned lds = (unsigned) (2 * 8 * score_entries(top_k));
-		const unsigned variant = held == SCORE_HELD_ROWS ? HIP_VARIANT_ROWS : held == SCORE_HELD_WIDE_ROWS ? HIP_VARIANT_WIDE_ROWS : HIP_VARIANT_LONG_ROWS;
+		const unsigned variant = held == SCORE_HELD_ROWS ? HIP_VARIANT_ROWS : held == SCORE_HELD_WIDE_ROWS ? HIP_VARIANT_WIDE_ROWS :
+								 held == SCORE_HELD_LONG_ROWS ? HIP_VARIANT_LONG_ROWS : HIP_VARIANT_ANY_ROWS;
 		set_1d(hip_launch_config, (unsigned) MY_MIN((long) n_rows, resident_groups(dataflow_handle, hip_function, variant, 64 * waves, lds)), (unsigned) (64 * waves), lds);
 		hip_launch_config->variant = variant;
 		return 0;

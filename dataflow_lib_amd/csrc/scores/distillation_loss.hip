@@ -451,6 +451,10 @@ __device__ __forceinline__ void distillation_loss_mean(int n_rows, const float *
 					 loss, dlogits, static_cast<Score_Part *>(workspace), nullptr};                                              \
 	a.picked = reinterpret_cast<float *>(a.parts + (uint64_t) n_rows * score_stream_plan(n_rows, n_cols, (int) sizeof(*logits), 0).slices);
 #define DISTILLATION_LOSS_KERNEL(SUF, T)                                                                                         \
+	extern "C" __global__ void __launch_bounds__(1024) distillation_loss_##SUF##_kernel_any_rows(DISTILLATION_ARGS(T)) { \
+		DISTILLATION_PACK \
+		distill_held<T, SCORE_HELD_MOST, 1024>(a); \
+	} \
 	extern "C" __global__ void __launch_bounds__(1024) distillation_loss_##SUF##_kernel_long_rows(DISTILLATION_ARGS(T)) { \
 		DISTILLATION_PACK \
 		distill_held<T, SCORE_HELD_MORE, 1024>(a); \

@@ -101,23 +101,27 @@ GEOM_FN unsigned long score_logprobs_workspace(int n_rows, int n_cols, int elem_
  * registers, with a thread per teacher entry. SCORE_HELD_ROWS: SCORE_HELD
  * chunks per thread in a wave or two (up to 16 where rows are few);
  * SCORE_HELD_WIDE_ROWS and SCORE_HELD_LONG_ROWS: SCORE_HELD_MORE chunks per
- * thread in up to 8 waves, and in 16. */
+ * thread in up to 8 waves, and in 16; SCORE_HELD_MOST_ROWS: SCORE_HELD_MOST in 16,
+ * all that its registers hold. */
 #define SCORE_HELD 4
 #define SCORE_HELD_MORE 16
+#define SCORE_HELD_MOST 20
 #define SCORE_HELD_FEW 512
 #define SCORE_HELD_NONE 0
 #define SCORE_HELD_ROWS 1
 #define SCORE_HELD_WIDE_ROWS 2
 #define SCORE_HELD_LONG_ROWS 3
+#define SCORE_HELD_MOST_ROWS 4
 GEOM_FN int score_held(int n_rows, int n_cols, int elem_bytes, int top_k) {
 	const long chunks = (long) n_cols * elem_bytes / 16;
 	if (chunks <= (n_rows <= SCORE_HELD_FEW ? 16 : 2) * 64 * SCORE_HELD) return SCORE_HELD_ROWS;
 	if (n_rows < SCORE_HELD_FEW / 4) return SCORE_HELD_NONE;
 	if (chunks <= 8 * 64 * SCORE_HELD_MORE && top_k <= 8 * 64) return SCORE_HELD_WIDE_ROWS;
-	return chunks <= 16 * 64 * SCORE_HELD_MORE ? SCORE_HELD_LONG_ROWS : SCORE_HELD_NONE;
+	if (chunks <= 16 * 64 * SCORE_HELD_MORE) return SCORE_HELD_LONG_ROWS;
+	return chunks <= 16 * 64 * SCORE_HELD_MOST ? SCORE_HELD_MOST_ROWS : SCORE_HELD_NONE;
 }
 GEOM_FN int score_held_waves(int held, int n_cols, int elem_bytes, int top_k) {
-	if (held == SCORE_HELD_LONG_ROWS) return 16;
+	if (held >= SCORE_HELD_LONG_ROWS) return 16;
 	const int chunks = (int) ((long) n_cols * elem_bytes / 16), per_wave = 64 * (held == SCORE_HELD_ROWS ? SCORE_HELD : SCORE_HELD_MORE);
 	const int waves = (chunks + per_wave - 1) / per_wave, entries = (top_k + 63) / 64;
 	return waves > entries ? waves : entries > 0 ? entries : 1;

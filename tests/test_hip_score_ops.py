@@ -471,7 +471,7 @@ def test_captured_and_replayed(hdl, shape):
 
 # each of the kernels that hold rows, with several rows to a workgroup: a wave,
 # a few waves, 16 waves
-WALKED = [(9001, 301, 0, 7), (800, 40001, 3, 30), (600, 66000, 0, 64)]
+WALKED = [(9001, 301, 0, 7), (800, 40001, 3, 30), (600, 66000, 0, 64), (530, 140003, 5, 20)]
 
 
 @pytest.mark.parametrize("dt", [BF16, FP16], ids=dt_id)
