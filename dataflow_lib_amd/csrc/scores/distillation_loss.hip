@@ -352,7 +352,8 @@ __device__ __forceinline__ void distill_parts(const DistillArgs & a) {
 			continue;
 		}
 		const RowSlice sl(a.n_cols, VecOf<T>::N, score_head(row, a.n_cols), slice, plan.slices, plan.slice_chunks);
-		const RowPart p = score_group_join<false>(score_stream<T, false, false>(row, sl, s_log2e, nullptr), s_log2e, cells);
+		const RowPart p = score_group_join<false>(a.dlogits ? score_stream<T, false, true>(row, sl, s_log2e, nullptr)
+																  : score_stream<T, false, false>(row, sl, s_log2e, nullptr), s_log2e, cells);
 		if (alone) {
 			distill_teacher(a, r, RowStats(p.m, p.z, 0.0f), true, te, cells, [&](int, uint32_t id) { return to_f(row[id]); });
 			continue;

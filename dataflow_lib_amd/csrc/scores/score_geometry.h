@@ -98,11 +98,18 @@ GEOM_FN unsigned long score_logprobs_workspace(int n_rows, int n_cols, int elem_
 }
 
 /* distillation_loss with a gradient: rows that a workgroup holds in its
- * registers, with a thread per teacher entry. SCORE_HELD_ROWS: SCORE_HELD
- * chunks per thread in a wave or two (up to 16 where rows are few);
- * SCORE_HELD_WIDE_ROWS and SCORE_HELD_LONG_ROWS: SCORE_HELD_MORE chunks per
- * thread in up to 8 waves, and in 16; SCORE_HELD_MOST_ROWS: SCORE_HELD_MOST in 16,
- * all that its registers hold. */
+ * registers, with a thread per teacher entry.
+ * - SCORE_HELD_ROWS: SCORE_HELD chunks per thread in a wave or two, 32 and 16
+ *   workgroups to a CU; up to 16 waves where rows are few (256 x 32000 bf16 13.3
+ *   us, with fewer waves of more chunks 21.0);
+ * - SCORE_HELD_WIDE_ROWS: SCORE_HELD_MORE chunks per thread in up to 8 waves, so
+ *   that two rows or more share a CU (8192 x 32000 bf16 208 us; 16 waves of
+ *   SCORE_HELD chunks, of which a CU has one workgroup, 365);
+ * - SCORE_HELD_LONG_ROWS, SCORE_HELD_MOST_ROWS: 16 waves of SCORE_HELD_MORE chunks,
+ *   and of SCORE_HELD_MOST, all that a CU's registers hold (2048 x 151936 bf16
+ *   249 us; read twice, 335);
+ * - longer rows, and a few of more than 8 waves, are cut into slices and read
+ *   twice (40 x 128256 bf16 19.7 us, held 22.9; 100 rows 32.3 and 23.3). */
 #define SCORE_HELD 4
 #define SCORE_HELD_MORE 16
 #define SCORE_HELD_MOST 20
@@ -115,8 +122,8 @@ GEOM_FN unsigned long score_logprobs_workspace(int n_rows, int n_cols, int elem_
 GEOM_FN int score_held(int n_rows, int n_cols, int elem_bytes, int top_k) {
 	const long chunks = (long) n_cols * elem_bytes / 16;
 	if (chunks <= (n_rows <= SCORE_HELD_FEW ? 16 : 2) * 64 * SCORE_HELD) return SCORE_HELD_ROWS;
-	if (n_rows < SCORE_HELD_FEW / 4) return SCORE_HELD_NONE;
 	if (chunks <= 8 * 64 * SCORE_HELD_MORE && top_k <= 8 * 64) return SCORE_HELD_WIDE_ROWS;
+	if (n_rows <= SCORE_HELD_FEW / 8) return SCORE_HELD_NONE;
 	if (chunks <= 16 * 64 * SCORE_HELD_MORE) return SCORE_HELD_LONG_ROWS;
 	return chunks <= 16 * 64 * SCORE_HELD_MOST ? SCORE_HELD_MOST_ROWS : SCORE_HELD_NONE;
 }

@@ -310,6 +310,31 @@ def test_largest_launches_stay_below_2_to_32_threads():
             assert rc == 0 and 0 < c.gridDimX * c.blockDimX < 2 ** 32, (op, rows, cols)
 
 
+def launched(op, dt, n_rows, n_cols, k, **change):
+    """(main kernel, kernel launched after it, finish kernel) of a call, by suffix"""
+    suffix = ["", "_rows", "_wide_rows", "_long_rows", "_multi", "_split", "_split_out", "_any_rows", "_top"]
+    change = dict(n_rows=n_rows, n_cols=n_cols, top_k=k, row_stride=n_cols, grad_stride=n_cols, logits=1 << 40, dlogits=1 << 50) | change
+    rc, c = config(op, dt, **change)
+    assert rc == 0
+    finish = op != "token_logprobs_bwd" and config(op, dt, finish=True, **change)[1].gridDimX > 0
+    return suffix[c.variant], suffix[c.then_variant], "_finish" if finish else ""
+
+
+@pytest.mark.parametrize("dt", DTS, ids=dt_id)
+def test_gpu_tests_reach_every_kernel(dt):
+    """one slice and several, with and without alternatives; rows held by each
+    of the kernels that hold them, and rows read twice"""
+    import test_hip_score_ops as T
+    logprobs = {launched("token_logprobs", dt, s[0], s[1], s[5]) for s in T.SHAPES}
+    assert logprobs == {("", "", ""), ("", "", "_finish"), ("_top", "", ""), ("_top", "", "_finish")}
+    distill = {launched("distillation_loss", dt, s[0], s[1], s[6], mean_loss=None)[:2] for s in T.KD_SHAPES}
+    walked = {launched("distillation_loss", dt, s[0], s[1], s[3], mean_loss=None)[:2] for s in T.WALKED}
+    held = {("_rows", ""), ("_wide_rows", ""), ("_long_rows", "")} | ({("_any_rows", "")} if dt != FP32 else set())
+    assert distill | walked >= held | {("", "_split_out")} and (dt == FP32 or walked == held)
+    alone = {launched("distillation_loss", dt, s[0], s[1], s[6], mean_loss=None, dlogits=None)[:2] for s in T.KD_SHAPES}
+    assert alone == {("", ""), ("", "_split_out")}
+
+
 def test_mean_loss_runs_only_where_it_is_wanted():
     assert config("distillation_loss", finish=True, mean_loss=None)[1].gridDimX == 0
     assert config("distillation_loss", finish=True)[1].gridDimX == 1
