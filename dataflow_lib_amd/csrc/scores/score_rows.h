@@ -11,8 +11,10 @@
  * moves its sums when that grows, from a to b:
  *   Z <- f Z,  E <- f (E + s (a - b) Z),  f = exp(s (a - b))
  * where all terms of E have one sign, so nothing cancels; threads, waves and
- * slices are joined in the same way, in a fixed order. Exponents are in units
- * of log 2 (t = s log2(e) (x - M)), and so is E until the end.
+ * slices are joined in the same way, in a fixed order: results do not change
+ * from call to call. Exponents are in units of log 2 (t = s log2(e) (x - M)),
+ * and so is E until the end. All of it is fp32; logits are widened exactly, and
+ * only gradients are rounded to their type, once.
  */
 #pragma once
 
@@ -166,8 +168,9 @@ __device__ __forceinline__ R16 score_load(const T * row, uint64_t uniform_chunk,
 
 /* A row's chunks begin where memory has a multiple of SCORE_ALIGN bytes, so
  * that a wave's accesses share no more lines with others than they have to
- * (rows of odd lengths begin anywhere: distillation_loss 4096 x 50257 bf16 198
- * -> 174 us, token_logprobs 4096 x 128257 216 -> 167 us). The elements before them, the head, and those behind the
+ * (rows of odd lengths begin anywhere: distillation_loss 4096 x 50257 bf16 174
+ * us, with chunks from the rows' first elements on 198; token_logprobs 4096 x
+ * 128257 167 and 216). The elements before them, the head, and those behind the
  * last whole chunk, the tail, are a thread's each (SCORE_ALIGN / 2 + 6 at
  * most, less than a wave). */
 #define SCORE_ALIGN 64
@@ -204,7 +207,7 @@ struct RowSlice {
 			if (t < head) return t;
 			t -= head;
 		}
-		return tail + t < end ? tail + t : -1;
+		return t < end - tail ? tail + t : -1;
 	}
 };
 
@@ -270,10 +273,14 @@ __device__ __forceinline__ float score_chunks(const T * row, int c, float s_log2
 }
 
 /* A thread's part of a slice: batches of SCORE_BATCH chunks, and what is left
- * in batches of half, a quarter and so on, so that only the last chunk has to
- * ask whether it is there. The maximum of the thread's b-th batch (what is left
- * being one) goes to groups[(b % SCORE_GROUP_SLOTS) * blockDim.x + tid] (LDS;
- * null: not wanted); AGAIN: some chunks are read again soon. The element behind the last whole chunk counts to batch 0. */
+ * in batches of 2 and 1, so that only the last chunk has to ask whether it is
+ * there. The maximum of the thread's b-th batch (what is left being one) goes
+ * to groups[(b % SCORE_GROUP_SLOTS) * blockDim.x + tid] (LDS; null: not
+ * wanted); the thread's element of the head or the tail counts to batch 0.
+ * AGAIN: the logits, or some of them, are read again soon, and come without the
+ * streaming hint (token_logprobs 1021 x 50257 bf16 with 64 alternatives 33.2 us,
+ * with the hint 41.3; distillation_loss of 300 x 128256 fp32, in two launches,
+ * 89 and 110). */
 template <typename T, bool ENTROPY, bool AGAIN>
 __device__ __forceinline__ RowPart score_stream(const T * row, const RowSlice & sl, float s_log2e, float * groups) {
 	const int nt = (int) blockDim.x, tid = (int) threadIdx.x;
@@ -297,7 +304,6 @@ __device__ __forceinline__ RowPart score_stream(const T * row, const RowSlice & 
 		}
 		else {
 			m = -__builtin_inff();
-			if (SCORE_BATCH > 4 && c + 4 * nt <= sl.last) { m = fmaxf(m, score_chunks<T, 4, ENTROPY, AGAIN>(row, c, s_log2e, p)); c += 4 * nt; }
 			if (c + 2 * nt <= sl.last) { m = fmaxf(m, score_chunks<T, 2, ENTROPY, AGAIN>(row, c, s_log2e, p)); c += 2 * nt; }
 			if (c + nt <= sl.last) { m = fmaxf(m, score_chunks<T, 1, ENTROPY, AGAIN>(row, c, s_log2e, p)); c += nt; }
 			if (c + tid < sl.last) m = fmaxf(m, score_chunks<T, 1, ENTROPY, AGAIN>(row, c, s_log2e, p));
@@ -346,7 +352,6 @@ __device__ __forceinline__ void score_map(const T * row, T * out, const RowSlice
 	out += sl.head;
 	int c = sl.first;
 	for (; c + SCORE_BATCH * nt <= sl.last; c += SCORE_BATCH * nt) score_map_chunks<T, SCORE_BATCH>(row, out, c, f);
-	if (SCORE_BATCH > 4 && c + 4 * nt <= sl.last) { score_map_chunks<T, 4>(row, out, c, f); c += 4 * nt; }
 	if (c + 2 * nt <= sl.last) { score_map_chunks<T, 2>(row, out, c, f); c += 2 * nt; }
 	if (c + nt <= sl.last) { score_map_chunks<T, 1>(row, out, c, f); c += nt; }
 	if (c + tid < sl.last) score_map_chunks<T, 1>(row, out, c, f);

@@ -277,7 +277,8 @@ def check_distill(dt, x, n_cols, scale, ids, v, wt, got):
 KD_SHAPES = [(1, 1, 0, 0, 0, 0, 1), (3, 2, 1, 0, 1, 0, 2), (5, 7, 0, 0, 0, 0, 4), (9, 65, 3, 1, 0, 0, 65), (33, 1000, 0, 0, 0, 0, 8), (300, 255, 0, 1, 3, 2, 5),
              (17, 2049, 0, 0, 5, 0, 32), (70, 8192, 0, 8, 0, 0, 1), (64, 32000, 64, 0, 0, 0, 10), (4, 50257, 0, 0, 0, 0, 1024), (600, 4099, 0, 0, 0, 1, 64),
              (2, 128256, 0, 0, 0, 0, 64), (1, 151937, 0, 0, 1, 0, 100), (3, 300001, 7, 0, 0, 0, 50), (2500, 300, 20, 4, 0, 0, 16), (130, 65536, 0, 0, 0, 0, 20),
-             (300, 131072, 0, 0, 0, 0, 16), (280, 65544, 0, 0, 8, 8, 64), (270, 32768, 0, 0, 0, 0, 128), (260, 131073, 0, 0, 0, 0, 3), (20, 70, 0, 0, 0, 0, 100)]
+             (300, 131072, 0, 0, 0, 0, 16), (280, 65544, 0, 0, 8, 8, 64), (270, 32768, 0, 0, 0, 0, 128), (260, 131073, 0, 0, 0, 0, 3), (20, 70, 0, 0, 0, 0, 100),
+             (70, 70001, 0, 0, 1, 0, 40)]
 
 
 @pytest.mark.parametrize("dt", DTS, ids=dt_id)
@@ -582,6 +583,47 @@ def test_a_row_of_more_than_4_gib(hdl):
         rounded_once(mid, BF16, pr, pr * 2.0 * slack, "the middle block")
         assert np.array_equal(np.delete(first, 7), np.delete(mid, 7)) and np.array_equal(np.delete(last, block - 2), np.delete(mid, block - 2))
         assert abs(to_f64(last, BF16)[block - 2] - (pr[block - 2] - q[0])) <= 2.0 ** -9 and abs(to_f64(first, BF16)[7] - (pr[7] - q[1])) <= 2.0 ** -9
+
+
+def test_a_row_of_all_the_columns_that_an_int_counts(hdl):
+    """2^31 - 1 columns that begin an element behind an aligned address: no
+    index passes 31 bits, and the element before the row stays"""
+    block, times, k = 1 << 24, 128, 3
+    n_cols = block * times - 1
+    x = logits(140, (1, block), block, BF16)
+    w = want_logprobs(BF16, x, block, 1.0, np.zeros((1, 1), np.uint32), k)
+    at = int(w["top_ids"][0][0])
+    assert at > 0
+    xf = to_f64(x, BF16)[0]
+    lse = w["lse"] + np.log(times - np.exp(xf[0] - w["lse"]))
+    with Dev(hdl) as d:
+        p = d.empty(2 * (n_cols + 1))
+        hdl.to_device(x, p)
+        for i in range(1, times):
+            assert hdl.copy(p + 2 * block * i, p, 2 * block) == 0
+        row = p + 2
+        ptok, plp, pe, pl, pi, pv, pg = d.put(np.array([[n_cols - 1]], np.uint32)), d.empty(4), d.empty(4), d.empty(4), d.empty(4 * k), d.empty(4 * k), d.put(np.ones((1, 1), np.float32))
+        s1 = space(d, api.token_logprobs_workspace(BF16, 1, n_cols, k))
+        assert api.submit_token_logprobs(hdl, 0, BF16, 1, n_cols, n_cols, 1.0, 1, k, row, ptok, plp, pe, pl, pi, pv, *s1) == 0
+        # 2^17 terms a thread, of four roundings each
+        slack = 2.0 ** 20 * U32
+        got_l = d.get(pl, (1,), np.float32)
+        close(got_l, lse, slack, "lse")
+        close(d.get(pe, (1,), np.float32), w["entropy"] + np.log(times), 20.0 * slack, "entropy")
+        close(d.get(plp, (1,), np.float32), xf[[block - 1]] - lse, slack, "logprobs")
+        assert np.array_equal(d.get(pi, (k,), np.uint32), (np.arange(k) * block + at - 1).astype(np.uint32))
+        ids, v, ploss = d.put(np.array([[n_cols - 1]], np.uint32)), d.put(np.ones((1, 1), np.float32)), d.empty(4)
+        s2 = space(d, api.distillation_loss_workspace(BF16, 1, n_cols, 1))
+        # one entry: the loss is minus its log-probability
+        assert api.submit_distillation_loss(hdl, 0, BF16, 1, n_cols, n_cols, n_cols, 1.0, 1, row, ids, v, None, ploss, None, None, *s2) == 0
+        close(d.get(ploss, (1,), np.float32), lse - xf[block - 1], slack, "loss")
+        assert api.submit_token_logprobs_bwd(hdl, 0, BF16, 1, n_cols, n_cols, n_cols, 1.0, 1, row, ptok, pl, None, pg, None, row) == 0
+        hdl.sync()
+        first, mid, last = [hdl.to_host(p + 2 * block * i, (block,), np.uint16) for i in (0, 64, times - 1)]
+        lp = xf - float(got_l[0])
+        rounded_once(mid, BF16, -np.exp(lp), np.exp(lp) * 4.0 * (4 * np.abs(lp) + 16) * U32, "the middle block")
+        assert np.array_equal(first[1:], mid[1:]) and first[0] == x[0, 0] and np.array_equal(last[:-1], mid[:-1])
+        assert abs(to_f64(last, BF16)[-1] - (1.0 - np.exp(lp[-1]))) <= 2.0 ** -8
 
 
 def test_rows_beyond_4_gib(hdl):

@@ -329,7 +329,7 @@ def test_gpu_tests_reach_every_kernel(dt):
     assert logprobs == {("", "", ""), ("", "", "_finish"), ("_top", "", ""), ("_top", "", "_finish")}
     distill = {launched("distillation_loss", dt, s[0], s[1], s[6], mean_loss=None)[:2] for s in T.KD_SHAPES}
     walked = {launched("distillation_loss", dt, s[0], s[1], s[3], mean_loss=None)[:2] for s in T.WALKED}
-    held = {("_rows", ""), ("_wide_rows", ""), ("_long_rows", "")} | ({("_any_rows", "")} if dt != FP32 else set())
+    held = {("_rows", ""), ("_wide_rows", ""), ("_long_rows", ""), ("_any_rows", "")}
     assert distill | walked >= held | {("", "_split_out")} and (dt == FP32 or walked == held)
     alone = {launched("distillation_loss", dt, s[0], s[1], s[6], mean_loss=None, dlogits=None)[:2] for s in T.KD_SHAPES}
     assert alone == {("", ""), ("", "_split_out")}
