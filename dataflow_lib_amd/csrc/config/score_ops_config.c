@@ -140,7 +140,6 @@ int token_logprobs_set_finish_launch_config(Hip_Launch_Config * hip_launch_confi
 	return 0;
 }
 
-
 int token_logprobs_bwd_set_launch_config(Hip_Launch_Config * hip_launch_config, Dataflow_Handle * dataflow_handle, Hip_Function * hip_function, Op * op) {
 	(void) dataflow_handle;
 	const char * what = "token logprobs bwd";

@@ -5,7 +5,14 @@
  *   dx_j = -s p_j (G + h (log p_j + H)) + s sum_m g_m [t_m = j].
  * Every column gets the first term; the tokens' columns, whose logits are set
  * aside before the first store (the gradient may lie in the logits' place),
- * are then stored once more, whole, so that they are rounded once.
+ * are then stored once more, whole, so that they are rounded once. p_j is
+ * exp(s x_j - lse) with the forward pass' lse, which is all that the row needs:
+ * nothing is reduced over columns.
+ *
+ * Bound by reading the logits and writing as much: 2048 x 128256 bf16 202 us
+ * (5.2 TB/s), 8192 x 32000 182 us (5.8 TB/s), 509 x 50257 fp16 22.0 us (4.7
+ * TB/s); 16 x 32000 fp32 5.5 us, a launch. Stores are aligned, loads lie as they
+ * do (8192 x 32001 186 us, with chunks from the rows' first elements on 223).
  */
 #include "score_rows.h"
 
