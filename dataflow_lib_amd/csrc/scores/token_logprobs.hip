@@ -16,10 +16,10 @@
  * Without alternatives: bound by reading the logits once, 16 bytes a thread and
  * four of them under way (4096 x 128256 bf16 159 us, 6.6 TB/s; 8 under way 167
  * us: half the waves fit). One exp2 and three operations per logit stay below
- * that. With them: 1021 x 50257 bf16, 64 alternatives, 34.1 us, of which the
- * bound, the second reading (out of L2), and the ranking, all of them latency,
- * are about a third; 6 waves to a SIMD, whose registers hold everything
- * (in 8 the compiler spills: 42.4 us; 5: 39.4). Few rows are bound by latency:
+ * that. With them: 1021 x 50257 bf16, 64 alternatives, 34.0 us, without 22.7:
+ * the bound, the second reading (out of L2) and the ranking are latency; 6
+ * waves to a SIMD, whose registers hold everything (in 8 the compiler spills:
+ * 42.4 us; 5: 39.4). Few rows are bound by latency:
  * 1 x 128256 with 20 alternatives 14.4 us, in two launches of about 5 us of host
  * time each, 64 x 128256 fp16 with 5 17.6 us.
  */
