@@ -29,8 +29,8 @@ struct GradTerm {
 	__device__ __forceinline__ float operator()(float x) const {
 		const float lp = fmaf(s, x, -lse);
 		const float p = __builtin_amdgcn_exp2f(lp * SCORE_LOG2E);
-		/* the bound keeps -inf * 0 out */
-		return p * (ENTROPY ? -s * fmaf(h, fmaxf(lp, -1e30f) + H, down) : -s * down);
+		/* the bound, below which p is 0, keeps -inf * 0 out */
+		return p * (ENTROPY ? -s * fmaf(h, fmaxf(lp, SCORE_FAR_BELOW) + H, down) : -s * down);
 	}
 };
 

@@ -227,6 +227,29 @@ def test_token_logprobs_bwd_of_odd_rows(hdl, dt, n_cols):
     assert not to_f64(out, dt)[[1, 6, 9]].any()
 
 
+@pytest.mark.parametrize("dt", [FP32, BF16], ids=dt_id)
+@pytest.mark.parametrize("scale, down", [(1.0, 1e9), (1e6, 1e4)])
+def test_large_gradients_of_masked_rows(hdl, dt, scale, down):
+    """columns of -inf get gradient 0 however large the entropy's gradient is"""
+    n_rows, n_cols = 3, 5003
+    x = logits(150, (n_rows, n_cols), n_cols, dt)
+    xf = to_f64(x, dt)
+    xf[:, ::3] = -np.inf
+    xf[:, 101] = xf[:, 100] = xf[np.isfinite(xf)].max() + 1.0   # two share all that the larger scale leaves
+    x = to_storage(xf.astype(np.float32), dt)
+    tok = tokens_for(151, n_rows, n_cols, 1)
+    lse, ent = forward_for(dt, x, n_cols, scale, tok)
+    g, he = normal_f32(152, (n_rows, 1)), np.float32(down) * np.array([1.0, -1.0, 0.5], np.float32)
+    out = run_grad(hdl, dt, x, n_cols, scale, tok, lse, ent, g, he)
+    o = to_f64(out, dt)
+    here = np.ones(n_cols, bool)
+    here[tok[tok < n_cols]] = False
+    assert np.isfinite(o).all() and not o[:, ~np.isfinite(xf[0]) & here].any()
+    if scale == 1.0:
+        v = want_grad(dt, x, n_cols, scale, tok, lse, ent, g, he)
+        rounded_once(out, dt, v, grad_slack(dt, x, n_cols, scale, tok, lse, ent, g, he), "dlogits")
+
+
 def test_gradient_against_differences(hdl):
     """the kernels alone: the loss through token_logprobs at shifted logits
     against token_logprobs_bwd, fp32"""
