@@ -196,7 +196,10 @@ int distillation_loss_set_launch_config(Hip_Launch_Config * hip_launch_config, D
 		hip_launch_config->variant = variant;
 		return 0;
 	}
-	const Score_Plan plan = score_stream_plan(n_rows, n_cols, (int) elem, 0);
+	Score_Plan plan = score_stream_plan(n_rows, n_cols, (int) elem, 0);
+	/* rows that are read and written, and too long to be held: as in
+	 * score_map_plan (2600 x 200000 bf16 549 -> 519 us) */
+	if (plan.slices == 1 && ARG(op, 12, void *)) plan.waves = 2 * SCORE_STREAM_WAVES;
 	plan_config(hip_launch_config, plan, n_rows, 0);
 	if (plan.slices > 1 || ARG(op, 12, void *)) hip_launch_config->then_variant = HIP_VARIANT_SPLIT_OUT;
 	return 0;

@@ -16,7 +16,7 @@
  * Bound by reading the logits and writing as much, held: 4096 x 128256 bf16 with
  * 64 entries 401 us (5.2 TB/s), 1024 x 50257 fp16 with 128 45.9 us (4.5 TB/s),
  * 8192 x 32000 207 us (5.1 TB/s); 2048 x 151936 249 us, read twice 335. Longer
- * rows are read twice: 2600 x 200000 550 us. The loss alone reads once: 256 x
+ * rows are read twice: 2600 x 200000 519 us. The loss alone reads once: 256 x
  * 151936 bf16 18.5 us with the mean, which is a launch of its own. Few rows are
  * bound by the launches: 1 x 128256 14.1 us, 7 x 1000 fp32 8.4 us.
  */

@@ -82,10 +82,17 @@ GEOM_FN Score_Plan score_stream_plan(int n_rows, int n_cols, int elem_bytes, int
 	return p;
 }
 
-/* the gradient kernels, which read and write a row once */
+/* token_logprobs_bwd, which reads and writes a row once. Rows that fill 16 waves
+ * with SCORE_BATCH chunks per thread take as many: fewer rows under way at once
+ * lie closer together, which reading with writing gains by (2048 x 128256 bf16
+ * 204 -> 190 us, 8192 x 16384 fp32 198 -> 187; shorter ones lose, 8192 x 16384
+ * bf16 93 -> 115 us, and so does reading alone: token_logprobs 4096 x 128256
+ * bf16 162 -> 171 us). */
 #define SCORE_MAP_WAVES 8
 GEOM_FN Score_Plan score_map_plan(int n_rows, int n_cols, int elem_bytes) {
-	return score_plan(n_rows, n_cols, elem_bytes, SCORE_MAP_BATCH, SCORE_MAP_WAVES);
+	Score_Plan p = score_plan(n_rows, n_cols, elem_bytes, SCORE_MAP_BATCH, SCORE_MAP_WAVES);
+	if (p.slices == 1 && p.slice_chunks >= 64 * SCORE_BATCH * 2 * SCORE_MAP_WAVES) p.waves = 2 * SCORE_MAP_WAVES;
+	return p;
 }
 
 /* what a slice of a row leaves in the workspace: its statistics, and its

@@ -9,8 +9,8 @@
  * exp(s x_j - lse) with the forward pass' lse, which is all that the row needs:
  * nothing is reduced over columns.
  *
- * Bound by reading the logits and writing as much: 2048 x 128256 bf16 202 us
- * (5.2 TB/s), 8192 x 32000 182 us (5.8 TB/s), 509 x 50257 fp16 22.0 us (4.7
+ * Bound by reading the logits and writing as much: 2048 x 128256 bf16 189 us
+ * (5.6 TB/s), 8192 x 32000 180 us (5.8 TB/s), 509 x 50257 fp16 22.0 us (4.7
  * TB/s); 16 x 32000 fp32 5.5 us, a launch. Stores are aligned, loads lie as they
  * do (8192 x 32001 186 us, with chunks from the rows' first elements on 223).
  */
@@ -106,7 +106,7 @@ __device__ __forceinline__ void token_logprobs_bwd_run(int n_rows, int n_cols, u
 }
 
 #define TOKEN_LOGPROBS_BWD_KERNEL(SUF, T)                                                                                      \
-	extern "C" __global__ void __launch_bounds__(64 * SCORE_MAP_WAVES) token_logprobs_bwd_##SUF##_kernel(int n_rows, int n_cols,      \
+	extern "C" __global__ void __launch_bounds__(64 * SCORE_MAX_WAVES, 8) token_logprobs_bwd_##SUF##_kernel(int n_rows, int n_cols,      \
 			uint64_t row_stride, uint64_t grad_stride, float scale, int tokens_per_row, T * logits, uint32_t * tokens,         \
 			float * lse, float * entropy, float * d_logprobs, float * d_entropy, T * dlogits) {                                \
 		token_logprobs_bwd_run<T>(n_rows, n_cols, row_stride, grad_stride, scale, tokens_per_row, logits, tokens, lse,         \
