@@ -14,8 +14,8 @@
  * slices and a second one reads them again for the gradient.
  *
  * Bound by reading the logits and writing as much, held: 4096 x 128256 bf16 with
- * 64 entries 401 us (5.2 TB/s), 1024 x 50257 fp16 with 128 45.9 us (4.5 TB/s),
- * 8192 x 32000 207 us (5.1 TB/s); 2048 x 151936 249 us, read twice 335. Longer
+ * 64 entries 365 us (5.8 TB/s), 1024 x 50257 fp16 with 128 45 us (4.5 TB/s),
+ * 8192 x 32000 205 us (5.1 TB/s); 2048 x 151936 230 us, read twice 335. Longer
  * rows are read twice: 2600 x 200000 519 us. The loss alone reads once: 256 x
  * 151936 bf16 18.5 us with the mean, which is a launch of its own. Few rows are
  * bound by the launches: 1 x 128256 14.1 us, 7 x 1000 fp32 8.4 us.
@@ -82,9 +82,11 @@ template <> __device__ __forceinline__ void buf_store_elem<bf16_t>(__amdgpu_buff
 #define SCORE_NOWHERE 0xfffffff0u
 
 /* A workgroup walks rows a grid apart and holds one of them: thread t has its
- * chunks t + j blockDim.x, j < CH. While a row's outputs are stored, each chunk's
- * registers take the next row's logits, so the next row arrives while this
- * one leaves and its statistics are formed as it arrives. All memory
+ * chunks t + j blockDim.x, j < CH. Behind a thread's last store of a row's outputs
+ * its registers take the next row's logits, so the next row arrives while this
+ * one leaves and its statistics are formed as it arrives. Stores and loads each
+ * go out together: memory does worse by them in turn (4096 x 128256 bf16 365 us;
+ * by fours 385, by ones 402). All memory
  * accesses are unconditional (buffer ranges drop what is not there), so the
  * waits count them exactly. Vector-memory operations complete in order, so
  * when a thread has a row's last chunk its stores of the row before are done;
@@ -266,8 +268,10 @@ __device__ __forceinline__ void distill_held(const DistillArgs & a) {
 #pragma unroll
 			for (int i = 0; i < V; i++) f[i] = grad(f[i]);
 			buf_store16_nt(ro, voff, (uint32_t) (j * nt) * 16u, pack16<T>(f));
-			x[j] = buf_load16_nt(rs, voff, (uint32_t) (j * nt) * 16u);
 		}
+		__builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+		for (int j = 0; j < CH; j++) x[j] = buf_load16_nt(rs, voff, (uint32_t) (j * nt) * 16u);
 		buf_store_elem<T>(make_rsrc(out, row_bytes), single, grad(xs));
 		head = next_head;
 		chunks = next_chunks;

@@ -114,11 +114,11 @@ GEOM_FN unsigned long score_logprobs_workspace(int n_rows, int n_cols, int elem_
  *   workgroups to a CU; up to 16 waves where rows are few (256 x 32000 bf16 13.3
  *   us, with fewer waves of more chunks 21.0);
  * - SCORE_HELD_WIDE_ROWS: SCORE_HELD_MORE chunks per thread in up to 8 waves, so
- *   that two rows or more share a CU (8192 x 32000 bf16 208 us; 16 waves of
+ *   that two rows or more share a CU (8192 x 32000 bf16 205 us; 16 waves of
  *   SCORE_HELD chunks, of which a CU has one workgroup, 365);
  * - SCORE_HELD_LONG_ROWS, SCORE_HELD_MOST_ROWS: 16 waves of SCORE_HELD_MORE chunks,
  *   and of SCORE_HELD_MOST, all that a CU's registers hold (2048 x 151936 bf16
- *   249 us; read twice, 335);
+ *   230 us; read twice, 335);
  * - longer rows, and a few of more than 8 waves, are cut into slices and read
  *   twice (40 x 128256 bf16 19.7 us, held 22.9; 100 rows 32.3 and 23.3). */
 #define SCORE_HELD 4
