@@ -71,14 +71,39 @@ GEOM_FN Score_Plan score_plan(int n_rows, int n_cols, int elem_bytes, int batch,
 	return p;
 }
 
-/* token_logprobs and the statistics of distillation_loss. Where no alternatives
- * are to be found, rows in one slice that would leave half of the chip's waves
+/* A wave of a workgroup that finds alternatives keeps so many maxima ("groups")
+ * per thread, and takes so many chunks per thread where rows are many. */
+#define SCORE_GROUP_SLOTS 4
+#define SCORE_TOP_CHUNKS 32
+#define SCORE_TOP_WAVES 2
+GEOM_FN long score_groups(int waves, long chunks) {
+	const long batches = (chunks + 64 * SCORE_BATCH * waves - 1) / (64 * SCORE_BATCH * waves);
+	return 64l * waves * (batches < SCORE_GROUP_SLOTS ? batches : SCORE_GROUP_SLOTS);
+}
+
+/* token_logprobs and the statistics of distillation_loss.
+ * With alternatives, whose second phase is latency, more rows at a time hide
+ * more of it: rows in one slice take SCORE_TOP_WAVES waves, or as many more as
+ * give a thread no more than SCORE_TOP_CHUNKS chunks and the chip
+ * SCORE_FILL_WAVES waves (bf16, 20 alternatives, next to up to 8 waves of
+ * SCORE_BATCH chunks: 8192 x 12000 127 -> 58 us, 8192 x 32000 150 -> 119, 8192 x
+ * 65000 216 -> 203); and, where there are as many chunks as alternatives, twice
+ * as many groups as alternatives (600 x 4096 with 100 95 -> 22 us).
+ * Where no alternatives are to be found, rows in one slice that would leave half of the chip's waves
  * free take workgroups of twice as many (256 x 151936 bf16 20.4 -> 18.5 us; with
  * alternatives, 300 x 32000 fp32, 17.6 -> 20.0). */
 GEOM_FN Score_Plan score_stream_plan(int n_rows, int n_cols, int elem_bytes, int top_k) {
 	Score_Plan p = score_plan(n_rows, n_cols, elem_bytes, SCORE_BATCH, SCORE_STREAM_WAVES);
 	if (top_k == 0 && p.slices == 1 && (long) n_rows * SCORE_STREAM_WAVES <= 2 * SCORE_FILL_WAVES && p.slice_chunks >= 64 * 4 * SCORE_STREAM_WAVES)
 		p.waves = 2 * SCORE_STREAM_WAVES;
+	if (top_k > 0 && p.slices == 1) {
+		const long chunks = p.slice_chunks;
+		int waves = SCORE_TOP_WAVES;
+		while (waves < p.waves && (64l * SCORE_TOP_CHUNKS * waves < chunks || (long) n_rows * waves < SCORE_FILL_WAVES)) waves *= 2;
+		if (waves > p.waves) waves = p.waves;
+		while (waves < SCORE_STREAM_WAVES && 64 * waves < chunks && chunks >= top_k && (64 * waves < top_k || score_groups(waves, chunks) < 2 * top_k)) waves *= 2;
+		p.waves = waves < SCORE_STREAM_WAVES ? waves : SCORE_STREAM_WAVES;
+	}
 	return p;
 }
 
@@ -157,7 +182,6 @@ GEOM_FN unsigned long score_distill_workspace(int n_rows, int n_cols, int elem_b
 
 /* token_logprobs: LDS of a workgroup with alternatives to find. Candidates,
  * group maxima (SCORE_GROUP_SLOTS per thread) and which of them reach a bound. */
-#define SCORE_GROUP_SLOTS 4
 #define SCORE_CANDIDATES 1024   /* all columns of a slice of so many */
 GEOM_FN unsigned score_top_lds(int waves) {
 	return (unsigned) (waves * 64 * SCORE_GROUP_SLOTS * 6 + SCORE_CANDIDATES * 8);

@@ -16,7 +16,7 @@
  * Without alternatives: bound by reading the logits once, 16 bytes a thread and
  * four of them under way (4096 x 128256 bf16 159 us, 6.6 TB/s; 8 under way 167
  * us: half the waves fit). One exp2 and three operations per logit stay below
- * that. With them: 1021 x 50257 bf16, 64 alternatives, 34.0 us, without 22.7:
+ * that. With them: 1021 x 50257 bf16, 64 alternatives, 32 us, without 22.7:
  * the bound, the second reading (out of L2) and the ranking are latency; 6
  * waves to a SIMD, whose registers hold everything (in 8 the compiler spills:
  * 42.4 us; 5: 39.4). Few rows are bound by latency:
@@ -195,12 +195,13 @@ __device__ __forceinline__ int score_candidates(const T * row, const RowSlice & 
 	float g[SCORE_GROUP_SLOTS];
 #pragma unroll
 	for (int i = 0; i < SCORE_GROUP_SLOTS; i++) g[i] = i < batches || i == 0 ? groups[i * nt + tid] : -__builtin_inff();
-	/* as many threads as have a column above -inf reach the least of their maxima */
+	/* as many threads as have a column above -inf reach the least of their maxima,
+	 * and most of their groups do */
 	float lo = least;
-	uint32_t reach = (uint32_t) met;
+	uint32_t reach = (uint32_t) met * (uint32_t) (batches < SCORE_GROUP_SLOTS ? batches > 1 ? batches : 1 : SCORE_GROUP_SLOTS);   /* groups, at most */
 	if (tid == 0) t.count = t.n_groups = 0u;
 	lds_barrier();
-	if (reach >= (uint32_t) k) {
+	if (met >= (float) k) {
 		lo = score_bound(lo, row_max, reach, k, [&](float mid) {
 			uint32_t n = 0;
 #pragma unroll

@@ -59,7 +59,7 @@ SHAPES = [(1, 1, 0, 0, 1, 1), (3, 2, 1, 1, 2, 2), (5, 7, 0, 0, 1, 7), (7, 64, 0,
           (17, 2049, 0, 5, 4, 64), (70, 8192, 0, 0, 1, 1), (5, 16385, 15, 0, 1, 128), (64, 32000, 64, 0, 4, 10), (4, 50257, 0, 0, 1, 256), (600, 4099, 0, 0, 1, 40),
           (2, 128256, 0, 0, 1, 20), (1, 151937, 0, 1, 1, 100), (3, 300001, 7, 0, 5, 256), (130, 65537, 0, 0, 1, 0), (257, 40000, 0, 0, 0, 3), (12, 131072, 0, 8, 1, 33),
           (2500, 300, 20, 0, 1, 7), (1, 1 << 21, 0, 0, 2, 50), (1, 1 << 21, 1, 0, 1, 256), (2, 128257, 0, 0, 3, 0), (60, 1000, 0, 0, 1, 256),
-          (90, 513, 0, 1, 1, 30)]
+          (90, 513, 0, 1, 1, 30), (1030, 6001, 1, 0, 1, 20), (600, 4096, 0, 0, 1, 100), (700, 20001, 0, 3, 1, 256), (2100, 1500, 0, 0, 2, 250)]
 
 
 @pytest.mark.parametrize("dt", DTS, ids=dt_id)
